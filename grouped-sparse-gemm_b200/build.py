@@ -18,7 +18,7 @@ OUT = os.path.join(HERE, "paired_nvfp4_kernels", "libpaired_nvfp4_b200.so")
 TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
 TORCH_OUT = os.path.join(HERE, "paired_nvfp4_kernels", "libpaired_nvfp4_torch.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "paired_nvfp4_b200.h")
-SOURCES = ["abi.cu", "quant.cu", "compress.cu", "routing.cu", "group_mm.cu"]
+SOURCES = ["abi.cu", "quant.cu", "compress.cu", "routing.cu", "group_mm.cu", "norm.cu", "route_topk.cu", "linear.cu"]
 
 
 def _inputs():

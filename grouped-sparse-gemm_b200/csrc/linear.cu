@@ -1,0 +1,887 @@
+// Dense linear layers: out = act(x w^T + bias) + residual, or act(gate) * up + residual where the rows of w hold gates and
+// ups in blocks of 32 (gated), on bf16 operands or on 8-bit codes with block scales (norm.cu says which).  The sum, the bias,
+// the activation and the residual are fp32, rounded once on the way out.
+//
+// Two kernels.
+//
+//   split    one CTA per 128 weight rows x 16 to 128 tokens, weight rows along the tensor core's M: token tiles as narrow
+//            as a decode step wants.  Where there are fewer tiles than SMs a cluster of up to eight CTAs shares a tile's K and
+//            adds its partial sums through distributed shared memory, in a fixed order: no workspace, no atomics.
+//   pair     persistent; a CTA pair multiplies 256 tokens x 256 weight rows with one instruction, tokens along M, so that a
+//            thread of the epilogue holds neighbouring features of one token.  Large products.
+//
+// Accumulation.  The tensor core adds to its fp32 accumulators with truncation: over K = 7168 the sums of random products
+// come out 7e-6 too small in magnitude (relative 8e-6, against 3e-7 of fp32 arithmetic).  That is nothing beside a rounding
+// to bf16, but not for float32 results (router logits), so the split kernel lets an accumulator grow over 512 K only and
+// adds those pieces in registers: 5e-7.
+//
+// Every mbarrier wait is bounded; one that gives up records a code in g_linear_status and the roles fall through to the end,
+// where tensor memory is freed.
+#include <cuda.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "common.cuh"
+#include "ptx.cuh"
+#include "tensor_map.cuh"
+
+namespace pnv {
+namespace {
+
+__device__ int g_linear_status = 0;
+enum LinearStatus : int { kLinProducer = 11, kLinMmaFull = 12, kLinMmaAcc = 13, kLinEpilogue = 14 };
+
+constexpr int kSmemMax = 227 * 1024;
+constexpr int kStageRow = 128;           // bytes of K per operand row and pipeline stage: one 128-byte swizzle row
+constexpr int kTileRows = 128;           // rows of one CTA's M operand
+constexpr int kABytes = kTileRows * kStageRow;
+constexpr int kBarBytes = 1024;
+
+struct LinearArgs {
+  void* out;
+  const void* bias;                      // or nullptr
+  const __nv_bfloat16* residual;         // or nullptr
+  const uint8_t* x_sf;                   // 8-bit operands
+  const uint8_t* w_sf;
+  long long residual_stride;
+  int rows, features, n_out;             // n_out: features, or half of them (gated)
+  int k_bytes;                           // bytes of K in a row of either operand
+  int m_tiles, n_tiles;                  // along tokens and along features
+  int out_f32, bias_f32, gated, kind;    // kind: PNV_ACT_*
+  GatedAct act;
+  int vec_out, vec_residual, vec_bias;   // how many bytes a vector access of these may have: 32, 16 or 0 (element by element)
+};
+
+// ---- epilogue arithmetic -------------------------------------------------------------------------
+
+__device__ __forceinline__ float silu_f32(float g) { return g * rcp_approx(1.f + ex2_approx(g * -kLog2e)); }
+
+template <int E>
+__device__ __forceinline__ void add_bias(float (&v)[E], const LinearArgs& a, int col) {
+  if (a.bias == nullptr) return;
+  if (a.bias_f32) {
+    const float* b = static_cast<const float*>(a.bias) + col;
+    if (a.vec_bias && col + E <= a.features) {
+#pragma unroll
+      for (int j = 0; j < E; j += 4) {
+        const float4 t = __ldg(reinterpret_cast<const float4*>(b + j));
+        v[j] += t.x; v[j + 1] += t.y; v[j + 2] += t.z; v[j + 3] += t.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (col + j < a.features) v[j] += __ldg(b + j);
+    }
+  } else {
+    const unsigned short* b = static_cast<const unsigned short*>(a.bias) + col;
+    if (a.vec_bias && col + E <= a.features) {
+#pragma unroll
+      for (int j = 0; j < E; j += 8) {
+        float f[8];
+        unpack8(__ldg(reinterpret_cast<const uint4*>(b + j)), f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j + i] += f[i];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (col + j < a.features) v[j] += __uint_as_float((uint32_t)__ldg(b + j) << 16);
+    }
+  }
+}
+
+template <int E>
+__device__ __forceinline__ void activate(float (&v)[E], const LinearArgs& a) {
+  switch (a.kind) {
+    case PNV_ACT_RELU:
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];        // (a NaN stays one)
+      break;
+    case PNV_ACT_SILU:
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = silu_f32(v[j]);
+      break;
+    case PNV_ACT_GELU:
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = 0.5f * v[j] * (1.f + erff(v[j] * 0.70710678f));
+      break;
+    default:
+      break;
+  }
+}
+
+template <int E>
+__device__ __forceinline__ void gate(const float (&g)[E], const float (&u)[E], float (&y)[E], const LinearArgs& a) {
+  if (a.kind == PNV_ACT_SITU) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) y[j] = situ_short(g[j], u[j], a.act.beta, a.act.inv_beta, a.act.linear_beta, a.act.inv_linear);
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j) y[j] = silu_f32(g[j]) * u[j];
+  }
+}
+
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
+// v: outputs col .. col + E - 1 of token `row`; the residual is added, then the one rounding.
+template <int E>
+__device__ __forceinline__ void store_outputs(float (&v)[E], const LinearArgs& a, int row, int col) {
+  static_assert(E == 8 || E == 16, "pieces of 8 or 16 outputs");
+  const bool whole = col + E <= a.n_out;
+  if (a.residual != nullptr) {
+    const __nv_bfloat16* r = a.residual + row * a.residual_stride + col;
+    if (a.vec_residual && whole) {
+#pragma unroll
+      for (int j = 0; j < E; j += 8) {
+        float f[8];
+        unpack8(__ldg(reinterpret_cast<const uint4*>(r + j)), f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j + i] += f[i];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (col + j < a.n_out) v[j] += __uint_as_float((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(r) + j) << 16);
+    }
+  }
+  if (a.out_f32) {
+    float* o = static_cast<float*>(a.out) + (long long)row * a.n_out + col;
+    if (a.vec_out && whole) {
+#pragma unroll
+      for (int j = 0; j < E; j += 4) *reinterpret_cast<float4*>(o + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (col + j < a.n_out) o[j] = v[j];
+    }
+    return;
+  }
+  uint32_t w[E / 2];
+#pragma unroll
+  for (int j = 0; j < E / 2; ++j) w[j] = as_u32(__floats2bfloat162_rn(v[2 * j], v[2 * j + 1]));
+  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + (long long)row * a.n_out + col;
+  if (whole && a.vec_out) {
+    if constexpr (E == 16) {
+      if (a.vec_out == 32) {
+        st_global_32(o, w);
+        return;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < E / 2; j += 4) *reinterpret_cast<uint4*>(o + 2 * j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (col + j < a.n_out) reinterpret_cast<unsigned short*>(o)[j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
+  }
+}
+
+// Instructions of a stage that meet any K at all (the last stage of a K that is no multiple of 128 bytes has fewer: blocks past
+// K are not multiplied, whatever scale they carry).
+__device__ __forceinline__ int stage_mmas(int k_bytes, int stage) { return min(4, (k_bytes - stage * kStageRow + 31) / 32); }
+
+// The four instructions of one stage; kMx8: the scale words of its four K-blocks sit at sfa and sfb.
+template <int CTAS, bool kMx8>
+__device__ __forceinline__ void issue_stage(uint32_t d, uint32_t a_smem, uint32_t b_smem, int n, int m, int mmas, bool first,
+                                            uint32_t sfa, uint32_t sfb) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < mmas) {
+      const uint64_t ad = ptx::smem_desc(a_smem + 32 * i, 1024, 16, 2), bd = ptx::smem_desc(b_smem + 32 * i, 1024, 16, 2);
+      const uint32_t accumulate = first && i == 0 ? 0u : 1u;
+      if constexpr (kMx8) ptx::tc_mma_mxf8<CTAS>(d, ad, bd, ptx::mma_mxf8_idesc(n, m, i), accumulate, sfa, sfb);
+      else ptx::tc_mma_bf16<CTAS>(d, ad, bd, ptx::mma_bf16_idesc(n, m), accumulate);
+    }
+  }
+}
+
+// After a wait gave up: time for the copies in flight to land before the CTA leaves.
+__device__ __forceinline__ void linger() {
+#pragma unroll 1
+  for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+}
+
+// ---- split kernel ----------------------------------------------------------------------------------
+
+template <int BN, bool kMx8>
+struct SplitCfg {
+  static_assert(BN == 16 || BN == 32 || BN == 64 || BN == 128, "token tiles of 16, 32, 64 or 128");
+  static constexpr int kGroups = BN >= 64 ? 2 : 1;                   // epilogue warps per quarter of the lanes
+  static constexpr int kEpiWarps = 4 * kGroups;
+  static constexpr int kThreads = (4 + kEpiWarps) * 32;              // producer, issuer, two idle warps, epilogue
+  static constexpr int kCols = BN / kGroups;                         // accumulator columns of an epilogue warp
+  static constexpr int kBBytes = BN * kStageRow;
+  static constexpr int kStageBytes = kABytes + kBBytes + (kMx8 ? 1024 : 0);
+  static constexpr int kMaxStages = 12;
+  static constexpr int kFit = (kSmemMax - 1024 - kBarBytes) / kStageBytes;
+  static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
+  static constexpr int kChunk = kMx8 ? 4 : 8;                        // stages an accumulator grows over: 512 K
+  static constexpr int kColSf = 2 * BN;                              // tensor memory: two accumulators, then the scales
+  static constexpr int kColsUsed = kColSf + (kMx8 ? 8 * kStages : 0);
+  static constexpr int kTmemCols = kColsUsed <= 32 ? 32 : kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
+  static constexpr int kPitch = kTileRows + 4;                       // floats between tokens of the partial sums
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kBarBytes;
+  static_assert(BN * kPitch * 4 <= kStages * kStageBytes, "the partial sums must fit the stages they take over");
+};
+
+template <int BN, bool kMx8>
+__global__ void __launch_bounds__(SplitCfg<BN, kMx8>::kThreads, 1)
+linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LinearArgs a,
+                    const int split) {
+  using C = SplitCfg<BN, kMx8>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* stages = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(stages + C::kStages * C::kStageBytes);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* acc_full = empty + C::kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = split > 1 ? (int)ptx::cluster_ctarank() : 0;
+  const int ft = (int)blockIdx.x / split, tt = (int)blockIdx.y;      // feature tile, token tile
+  if (warp == 0) {
+    if (ptx::elect_one()) {
+      ptx::prefetch_tensormap(&map_w);
+      ptx::prefetch_tensormap(&map_x);
+      for (int s = 0; s < C::kStages; ++s) {
+        ptx::mbar_init(full + s, 1);
+        ptx::mbar_init(empty + s, 1);
+      }
+      for (int b = 0; b < 2; ++b) {
+        ptx::mbar_init(acc_full + b, 1);
+        ptx::mbar_init(acc_empty + b, C::kEpiWarps);
+      }
+      ptx::fence_mbar_init();
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    ptx::tmem_alloc(tmem_slot, C::kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const int k_stages = (a.k_bytes + kStageRow - 1) / kStageRow;
+  const int ks0 = (int)((long long)rank * k_stages / split), ks1 = (int)((long long)(rank + 1) * k_stages / split);
+  const int chunks = (ks1 - ks0 + C::kChunk - 1) / C::kChunk;
+  float sum[C::kCols];
+  if (warp == 0) {
+    // ---- producer
+    const int n_kt = k_stages;           // an atom of scales has the 128 codes of a stage
+    int stage = 0;
+    uint32_t phase = 0;
+#pragma unroll 1
+    for (int ks = ks0; ks < ks1; ++ks) {
+      if (!ptx::mbar_wait_warp(empty + stage, phase ^ 1)) {
+        atomicExch(&g_linear_status, kLinProducer);
+        linger();
+        break;
+      }
+      uint8_t* st = stages + stage * C::kStageBytes;
+      if (ptx::elect_one()) {
+        ptx::mbar_arrive_expect_tx(full + stage, C::kStageBytes);
+        ptx::tma_load_3d(st, &map_w, full + stage, ks * kStageRow, ft * kTileRows, 0);
+        ptx::tma_load_3d(st + kABytes, &map_x, full + stage, ks * kStageRow, tt * BN, 0);
+        if constexpr (kMx8) {            // (a token tile below 128 is the only one and starts its atom)
+          ptx::bulk_load(st + kABytes + C::kBBytes, a.w_sf + ((long long)ft * n_kt + ks) * 512, 512, full + stage);
+          ptx::bulk_load(st + kABytes + C::kBBytes + 512, a.x_sf + ((long long)tt * n_kt + ks) * 512, 512, full + stage);
+        }
+      }
+      __syncwarp();
+      if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+    }
+  } else if (warp == 1) {
+    // ---- issuer
+    int stage = 0;
+    uint32_t phase = 0;
+#pragma unroll 1
+    for (int ks = ks0; ks < ks1; ++ks) {
+      const int done = ks - ks0, chunk = done / C::kChunk, buf = chunk & 1;
+      const bool first = done % C::kChunk == 0;
+      if (first && !ptx::mbar_wait_warp(acc_empty + buf, ((chunk >> 1) & 1) ^ 1)) {
+        atomicExch(&g_linear_status, kLinMmaAcc);
+        break;
+      }
+      if (!ptx::mbar_wait_warp(full + stage, phase)) {
+        atomicExch(&g_linear_status, kLinMmaFull);
+        break;
+      }
+      ptx::tc_fence_after();
+      const uint32_t st = ptx::smem_u32(stages + stage * C::kStageBytes);
+      if (ptx::elect_one()) {
+        const uint32_t sfa = tmem + C::kColSf + 8 * stage, sfb = sfa + 4;
+        if constexpr (kMx8) {
+          ptx::tc_cp_32x128b_warpx4(sfa, ptx::smem_desc(st + kABytes + C::kBBytes, 128, 0, 0));
+          ptx::tc_cp_32x128b_warpx4(sfb, ptx::smem_desc(st + kABytes + C::kBBytes + 512, 128, 0, 0));
+        }
+        issue_stage<1, kMx8>(tmem + buf * BN, st, st + kABytes, BN, kTileRows, stage_mmas(a.k_bytes, ks), first, sfa, sfb);
+        ptx::tc_commit(empty + stage);
+        if ((done + 1) % C::kChunk == 0 || ks + 1 == ks1) ptx::tc_commit(acc_full + buf);
+      }
+      __syncwarp();
+      if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue: the pieces of 512 K are added in registers
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;                 // lane quarter of this warp
+    const int col0 = (warp - 4) / 4 * C::kCols;
+#pragma unroll
+    for (int j = 0; j < C::kCols; ++j) sum[j] = 0.f;
+#pragma unroll 1
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+      const int buf = chunk & 1;
+      if (!ptx::mbar_wait_warp(acc_full + buf, (chunk >> 1) & 1)) {
+        atomicExch(&g_linear_status, kLinEpilogue);
+        break;
+      }
+      ptx::tc_fence_after();
+      const uint32_t src = tmem + lanes + buf * BN + col0;
+      if constexpr (C::kCols == 16) {
+        uint32_t r[16];
+        ptx::tc_ld_32x16(src, r);
+        ptx::tc_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[j] += __uint_as_float(r[j]);
+      } else {
+#pragma unroll
+        for (int h = 0; h < C::kCols; h += 32) {
+          uint32_t r[32];
+          ptx::tc_ld_32x32(src + h, r);
+          ptx::tc_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sum[h + j] += __uint_as_float(r[j]);
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(acc_empty + buf);
+    }
+    // every load and product of this CTA is over: the stages' memory takes the sums, [token][feature]
+    float* part = reinterpret_cast<float*>(stages) + col0 * C::kPitch + (warp & 3) * 32 + lane;
+#pragma unroll
+    for (int j = 0; j < C::kCols; ++j) part[j * C::kPitch] = sum[j];
+  }
+  __syncwarp();
+  if (split > 1) ptx::cluster_sync(); else __syncthreads();
+
+  // ---- the CTAs of the cluster share the tile's outputs, in pieces of eight neighbouring features of a token
+  {
+    const int tokens = min(BN, a.rows - tt * BN);
+    const int per_token = a.gated ? 8 : 16;
+    const int units = tokens * per_token, share = (units + split - 1) / split;
+    const int end = min(units, (rank + 1) * share);
+    const float* part = reinterpret_cast<const float*>(stages);
+    for (int u = rank * share + (int)threadIdx.x; u < end; u += C::kThreads) {
+      const int token = u / per_token, piece = u - token * per_token;
+      // gated: features [64 b, 64 b + 32) are gates, the next 32 their ups
+      const int f = a.gated ? (piece >> 2) * 64 + (piece & 3) * 8 : piece * 8;
+      const int col = ft * kTileRows + f;
+      if (col >= a.features) continue;
+      float v[8], up[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = up[j] = 0.f;
+      const float* src = part + token * C::kPitch + f;
+      for (int r = 0; r < split; ++r) {
+        const float4 p = split > 1 ? ptx::ld_cluster_f4(src, r) : *reinterpret_cast<const float4*>(src);
+        const float4 q = split > 1 ? ptx::ld_cluster_f4(src + 4, r) : *reinterpret_cast<const float4*>(src + 4);
+        v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
+        v[4] += q.x; v[5] += q.y; v[6] += q.z; v[7] += q.w;
+        if (a.gated) {
+          const float4 s = split > 1 ? ptx::ld_cluster_f4(src + 32, r) : *reinterpret_cast<const float4*>(src + 32);
+          const float4 t = split > 1 ? ptx::ld_cluster_f4(src + 36, r) : *reinterpret_cast<const float4*>(src + 36);
+          up[0] += s.x; up[1] += s.y; up[2] += s.z; up[3] += s.w;
+          up[4] += t.x; up[5] += t.y; up[6] += t.z; up[7] += t.w;
+        }
+      }
+      add_bias(v, a, col);
+      if (a.gated) {
+        add_bias(up, a, col + 32);
+        float y[8];
+        gate(v, up, y, a);
+        store_outputs(y, a, tt * BN + token, (col - f) / 2 + (piece >> 2) * 32 + (piece & 3) * 8);
+      } else {
+        activate(v, a);
+        store_outputs(v, a, tt * BN + token, col);
+      }
+    }
+  }
+  ptx::tc_fence_before();
+  if (split > 1) ptx::cluster_sync(); else __syncthreads();         // (no CTA leaves while its sums are being read)
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+// ---- pair kernel -----------------------------------------------------------------------------------
+
+template <bool kMx8>
+struct PairCfg {
+  static constexpr int kTileM = 256, kTileN = 256;                   // tokens and features of a pair's tile
+  static constexpr int kEpiWarps = 16;
+  static constexpr int kThreads = (4 + kEpiWarps) * 32;
+  static constexpr int kBBytes = 128 * kStageRow;                    // half of the features
+  static constexpr int kSfBytes = kMx8 ? 512 + 1024 : 0;             // own tokens' scales, all features' scales
+  static constexpr int kStageBytes = kABytes + kBBytes + (kMx8 ? 2048 : 0);
+  static constexpr int kStages = (kSmemMax - 1024 - kBarBytes) / kStageBytes;
+  static constexpr int kLoadBytes = 2 * (kABytes + kBBytes + kSfBytes);
+  // 8-bit operands: the scale words need columns, so there is one accumulator; its readers hand it back as soon as they
+  // have it in registers
+  static constexpr int kAccs = kMx8 ? 1 : 2;
+  static constexpr int kColSf = kAccs * kTileN;
+  static constexpr int kTmemCols = 512;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kBarBytes;
+  static_assert(kColSf + (kMx8 ? 12 * kStages : 0) <= kTmemCols, "tensor-memory column map overflows");
+};
+
+// Tiles in bands of eight along the tokens (2048 of them), features outer within a band: the tiles that run at one time share
+// activations and weights in L2.
+constexpr int kBand = 8;
+__device__ __forceinline__ void pair_tile(int tile, int m_tiles, int n_tiles, int& mt, int& nt) {
+  const int band = tile / (kBand * n_tiles), in = tile - band * kBand * n_tiles;
+  const int height = min(kBand, m_tiles - band * kBand);
+  nt = in / height;
+  mt = band * kBand + in - nt * height;
+}
+
+template <bool kMx8>
+__global__ void __launch_bounds__(PairCfg<kMx8>::kThreads, 1)
+linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                   const __grid_constant__ CUtensorMap map_w_sf, const __grid_constant__ CUtensorMap map_x_sf, const LinearArgs a) {
+  using C = PairCfg<kMx8>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* stages = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(stages + C::kStages * C::kStageBytes);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* acc_full = empty + C::kStages;
+  uint64_t* acc_empty = acc_full + C::kAccs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + C::kAccs);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();
+  if (warp == 0) {
+    if (ptx::elect_one()) {
+      ptx::prefetch_tensormap(&map_w);
+      ptx::prefetch_tensormap(&map_x);
+      for (int s = 0; s < C::kStages; ++s) {
+        ptx::mbar_init(full + s, 1);
+        ptx::mbar_init(empty + s, 1);
+      }
+      for (int b = 0; b < C::kAccs; ++b) {
+        ptx::mbar_init(acc_full + b, 1);
+        ptx::mbar_init(acc_empty + b, 2 * C::kEpiWarps);
+      }
+      ptx::fence_mbar_init();
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    ptx::tmem_alloc<2>(tmem_slot, C::kTmemCols);
+    ptx::tmem_relinquish<2>();
+  }
+  ptx::tc_fence_before();
+  ptx::cluster_sync();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const int k_stages = (a.k_bytes + kStageRow - 1) / kStageRow;
+  const int tiles = a.m_tiles * a.n_tiles, pairs = (int)gridDim.x / 2;
+  if (warp == 0) {
+    // ---- producer, in both CTAs: own tokens, own half of the features; completion is counted on the first CTA's barrier
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int tile = (int)blockIdx.x / 2; ok && tile < tiles; tile += pairs) {
+      int mt, nt;
+      pair_tile(tile, a.m_tiles, a.n_tiles, mt, nt);
+#pragma unroll 1
+      for (int ks = 0; ks < k_stages; ++ks) {
+        if (!ptx::mbar_wait_warp(empty + stage, phase ^ 1)) {
+          atomicExch(&g_linear_status, kLinProducer);
+          ok = false;
+          break;
+        }
+        uint8_t* st = stages + stage * C::kStageBytes;
+        if (ptx::elect_one()) {
+          if (rank == 0) ptx::mbar_arrive_expect_tx(full + stage, C::kLoadBytes);
+          ptx::tma_load_3d_pair(st, &map_x, full + stage, 0, ks * kStageRow, mt * 256 + (int)rank * 128, 0);
+          ptx::tma_load_3d_pair(st + kABytes, &map_w, full + stage, 0, ks * kStageRow, nt * 256 + (int)rank * 128, 0);
+          if constexpr (kMx8) {
+            ptx::tma_load_3d_pair(st + kABytes + C::kBBytes, &map_x_sf, full + stage, 0, 0, ks, mt * 2 + (int)rank);
+            ptx::tma_load_3d_pair(st + kABytes + C::kBBytes + 512, &map_w_sf, full + stage, 0, 0, ks, nt * 2);
+          }
+        }
+        __syncwarp();
+        if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+      }
+    }
+    if (!ok) linger();
+  } else if (warp == 1 && rank == 0) {
+    // ---- issuer
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int tile = (int)blockIdx.x / 2; ok && tile < tiles; tile += pairs) {
+      if (!ptx::mbar_wait_warp(acc_empty + acc, acc_phase ^ 1)) {
+        atomicExch(&g_linear_status, kLinMmaAcc);
+        break;
+      }
+      ptx::tc_fence_after();
+#pragma unroll 1
+      for (int ks = 0; ks < k_stages; ++ks) {
+        if (!ptx::mbar_wait_warp(full + stage, phase)) {
+          atomicExch(&g_linear_status, kLinMmaFull);
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t st = ptx::smem_u32(stages + stage * C::kStageBytes);
+        if (ptx::elect_one()) {
+          const uint32_t sfa = tmem + C::kColSf + 12 * stage, sfb = sfa + 4;
+          if constexpr (kMx8) {
+            const uint32_t sf = st + kABytes + C::kBBytes;
+            ptx::tc_cp_32x128b_warpx4<2>(sfa, ptx::smem_desc(sf, 128, 0, 0));
+            ptx::tc_cp_32x128b_warpx4<2>(sfb, ptx::smem_desc(sf + 512, 128, 0, 0));
+            ptx::tc_cp_32x128b_warpx4<2>(sfb + 4, ptx::smem_desc(sf + 1024, 128, 0, 0));
+          }
+          issue_stage<2, kMx8>(tmem + acc * C::kTileN, st, st + kABytes, C::kTileN, C::kTileM, stage_mmas(a.k_bytes, ks), ks == 0, sfa, sfb);
+          ptx::tc_commit_pair(empty + stage);
+          if (ks + 1 == k_stages) ptx::tc_commit_pair(acc_full + acc);
+        }
+        __syncwarp();
+        if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+      }
+      if (++acc == C::kAccs) { acc = 0; acc_phase ^= 1; }
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue: a thread has 64 neighbouring features of one token
+    const int quarter = warp & 3, group = (warp - 4) >> 2;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+#pragma unroll 1
+    for (int tile = (int)blockIdx.x / 2; tile < tiles; tile += pairs) {
+      int mt, nt;
+      pair_tile(tile, a.m_tiles, a.n_tiles, mt, nt);
+      if (!ptx::mbar_wait_warp(acc_full + acc, acc_phase)) {
+        atomicExch(&g_linear_status, kLinEpilogue);
+        break;
+      }
+      ptx::tc_fence_after();
+      uint32_t r[2][32];
+      const uint32_t src = tmem + ((uint32_t)quarter << 21) + acc * C::kTileN + group * 64;
+      ptx::tc_ld_32x32(src, r[0]);
+      ptx::tc_ld_32x32(src + 32, r[1]);
+      ptx::tc_ld_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(acc_empty + acc, 0);
+      if (++acc == C::kAccs) { acc = 0; acc_phase ^= 1; }
+      const int row = mt * 256 + (int)rank * 128 + quarter * 32 + lane;
+      const int col = nt * 256 + group * 64;
+      const bool live = row < a.rows && col < a.features;
+      if (live && a.gated) {
+#pragma unroll
+        for (int h = 0; h < 32; h += 16) {
+          float g[16], u[16], y[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) { g[j] = __uint_as_float(r[0][h + j]); u[j] = __uint_as_float(r[1][h + j]); }
+          add_bias(g, a, col + h);
+          add_bias(u, a, col + 32 + h);
+          gate(g, u, y, a);
+          store_outputs(y, a, row, col / 2 + h);
+        }
+      } else if (live) {
+#pragma unroll
+        for (int h = 0; h < 64; h += 16) {
+          if (col + h < a.features) {
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[h / 32][h % 32 + j]);
+            add_bias(v, a, col + h);
+            activate(v, a);
+            store_outputs(v, a, row, col + h);
+          }
+        }
+      }
+      __syncwarp();
+    }
+  }
+  __syncwarp();
+  ptx::tc_fence_before();
+  ptx::cluster_sync();                   // (the partner's barriers and tensor memory are in use until both are here)
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<2>(tmem, C::kTmemCols);
+  }
+}
+
+// ---- host side -------------------------------------------------------------------------------------
+
+MapCache g_linear_maps;
+
+// An operand [rows][k_bytes], rows `stride` bytes apart, in boxes of box_rows x 128 bytes (128-byte swizzle).
+int operand_map(CUtensorMap* map, const void* base, uint64_t k_bytes, uint64_t rows, uint64_t stride, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  return cached_map(g_linear_maps, map, MapKey{base, k_bytes, rows, stride, box_rows, kStageRow, 0u}, [&](CUtensorMap* m) {
+    cuuint64_t dims[3] = {k_bytes, rows, 1};
+    cuuint64_t strides[2] = {stride, stride * rows};
+    cuuint32_t box[3] = {kStageRow, box_rows, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+      return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled (operand) failed with CUresult %d (row_bytes=%llu rows=%llu)", (int)r,
+                  (unsigned long long)k_bytes, (unsigned long long)rows);
+    return (int)PNV_OK;
+  });
+}
+
+// A scale buffer as [row atoms][K atoms][128 words], in boxes of `atoms` row atoms of one K atom.  (A tiled copy, unlike a
+// plain bulk copy, can count its bytes on the partner's barrier.)
+int scale_map(CUtensorMap* map, const void* base, uint64_t row_atoms, uint64_t k_atoms, uint32_t atoms) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  return cached_map(g_linear_maps, map, MapKey{base, k_atoms, row_atoms, 0, atoms, 128, 1u}, [&](CUtensorMap* m) {
+    cuuint64_t dims[3] = {128, k_atoms, row_atoms};
+    cuuint64_t strides[2] = {512, 512 * k_atoms};
+    cuuint32_t box[3] = {128, 1, atoms};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+      return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled (scales) failed with CUresult %d (row atoms=%llu, K atoms=%llu)", (int)r,
+                  (unsigned long long)row_atoms, (unsigned long long)k_atoms);
+    return (int)PNV_OK;
+  });
+}
+
+constexpr int kMaxSplitLog = 3;          // clusters of 1, 2, 4 or 8 CTAs
+
+// Per kernel and device, once: shared-memory carve-out, and how many clusters of each size run at one time.
+struct Setup {
+  std::once_flag once[64];
+  cudaError_t err[64] = {};
+  int clusters[64][kMaxSplitLog + 1] = {};
+};
+
+template <class Kernel>
+int prepare(Kernel kernel, Setup& s, int threads, size_t smem, const int** clusters) {
+  int dev = 0;
+  PNV_CUDA(cudaGetDevice(&dev));
+  PNV_REQUIRE(dev >= 0 && dev < 64, "unexpected CUDA device index %d", dev);
+  std::call_once(s.once[dev], [&] {
+    s.err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    for (int i = 0; i <= kMaxSplitLog && s.err[dev] == cudaSuccess; ++i) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(8 << 7);
+      cfg.blockDim = dim3(threads);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1u << i;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      s.err[dev] = cudaOccupancyMaxActiveClusters(&s.clusters[dev][i], kernel, &cfg);
+    }
+  });
+  if (s.err[dev] != cudaSuccess) return fail(PNV_ERR_CUDA, "linear kernel set-up failed: %s", cudaGetErrorString(s.err[dev]));
+  *clusters = s.clusters[dev];
+  return PNV_OK;
+}
+
+template <class Kernel, class... Args>
+cudaError_t launch_clusters(Kernel kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+struct Operands {
+  const void* x;
+  const void* w;
+  long long x_stride;                    // bytes
+};
+
+template <int BN, bool kMx8>
+int split_setup(const int** clusters) {
+  static Setup setup;
+  return prepare(linear_split_kernel<BN, kMx8>, setup, SplitCfg<BN, kMx8>::kThreads, SplitCfg<BN, kMx8>::kSmem, clusters);
+}
+template <bool kMx8>
+int pair_setup(const int** clusters) {
+  static Setup setup;
+  return prepare(linear_pair_kernel<kMx8>, setup, PairCfg<kMx8>::kThreads, PairCfg<kMx8>::kSmem, clusters);
+}
+
+template <int BN, bool kMx8>
+int launch_split(const Operands& o, const LinearArgs& a, int split, cudaStream_t stream) {
+  using C = SplitCfg<BN, kMx8>;
+  CUtensorMap map_w, map_x;
+  if (int rc = operand_map(&map_w, o.w, a.k_bytes, a.features, a.k_bytes, kTileRows)) return rc;
+  if (int rc = operand_map(&map_x, o.x, a.k_bytes, a.rows, o.x_stride, BN)) return rc;
+  const dim3 grid((unsigned)(ceil_div_i(a.features, kTileRows) * split), (unsigned)ceil_div_i(a.rows, BN));
+  PNV_CUDA(launch_clusters(linear_split_kernel<BN, kMx8>, grid, C::kThreads, C::kSmem, split, stream, map_w, map_x, a, split));
+  return PNV_OK;
+}
+
+template <bool kMx8>
+int launch_pair(const Operands& o, const LinearArgs& a, int pairs, cudaStream_t stream) {
+  using C = PairCfg<kMx8>;
+  CUtensorMap map_w, map_x, map_w_sf = {}, map_x_sf = {};
+  if (int rc = operand_map(&map_w, o.w, a.k_bytes, a.features, a.k_bytes, 128)) return rc;
+  if (int rc = operand_map(&map_x, o.x, a.k_bytes, a.rows, o.x_stride, 128)) return rc;
+  if (kMx8) {
+    const int k_atoms = ceil_div_i(a.k_bytes, 128);
+    if (int rc = scale_map(&map_w_sf, a.w_sf, sf_row_atoms(a.features), k_atoms, 2)) return rc;
+    if (int rc = scale_map(&map_x_sf, a.x_sf, sf_row_atoms(a.rows), k_atoms, 1)) return rc;
+  }
+  PNV_CUDA(launch_clusters(linear_pair_kernel<kMx8>, dim3((unsigned)(2 * pairs)), C::kThreads, C::kSmem, 2, stream, map_w, map_x, map_w_sf,
+                           map_x_sf, a));
+  return PNV_OK;
+}
+
+// Which kernel, and how many CTAs share a tile's K.
+template <bool kMx8>
+int run_linear(const Operands& o, LinearArgs a, int sm_count, cudaStream_t stream) {
+  const int k_stages = ceil_div_i(a.k_bytes, kStageRow);
+  const int bn = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : a.rows <= 64 ? 64 : 128;
+  const long long tiles = (long long)ceil_div_i(a.features, kTileRows) * ceil_div_i(a.rows, bn);
+  const int* clusters = nullptr;
+  if (int rc = bn == 16 ? split_setup<16, kMx8>(&clusters) : bn == 32 ? split_setup<32, kMx8>(&clusters)
+             : bn == 64 ? split_setup<64, kMx8>(&clusters) : split_setup<128, kMx8>(&clusters))
+    return rc;
+  int split = 1;
+  for (int i = 1; i <= kMaxSplitLog; ++i)
+    if (tiles <= std::min(clusters[i], sm_count >> i) && (k_stages >> i) >= 2) split = 1 << i;
+  if (!a.out_f32 && bn == 128) {
+    const int* pair_clusters = nullptr;
+    if (int rc = pair_setup<kMx8>(&pair_clusters)) return rc;
+    const int pairs = std::min(pair_clusters[1], sm_count / 2);
+    const long long m_tiles = ceil_div_i(a.rows, 256), n_tiles = ceil_div_i(a.features, 256), pair_tiles = m_tiles * n_tiles;
+    // A stage of a 128 x 128 tile and one of a 256 x 256 tile of a pair take about as long: both are bound by what a CTA
+    // takes in from L2, which is the same 32 KB.
+    const long long split_waves = (tiles * split + sm_count - 1) / sm_count;
+    if (pairs >= 1 && pair_tiles < (1LL << 31) / kBand && (pair_tiles + pairs - 1) / pairs * split <= split_waves) {
+      a.m_tiles = (int)m_tiles;
+      a.n_tiles = (int)n_tiles;
+      return launch_pair<kMx8>(o, a, (int)std::min<long long>(pairs, pair_tiles), stream);
+    }
+  }
+  PNV_REQUIRE(ceil_div_i(a.rows, bn) <= 65535 && ceil_div_i(a.features, kTileRows) < (1 << 28), "linear: too many rows for one call");
+  switch (bn) {
+    case 16: return launch_split<16, kMx8>(o, a, split, stream);
+    case 32: return launch_split<32, kMx8>(o, a, split, stream);
+    case 64: return launch_split<64, kMx8>(o, a, split, stream);
+    default: return launch_split<128, kMx8>(o, a, split, stream);
+  }
+}
+
+bool at(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int linear_common(bool mx8, void* out, int out_is_f32, const void* x, long long x_stride, const uint8_t* x_sf, const void* w, const uint8_t* w_sf,
+                  const void* bias, int bias_is_f32, const void* residual, long long residual_stride, long long rows, int features, int k,
+                  int act_kind, int gated, float beta, float linear_beta, int sm_count, cudaStream_t stream) {
+  PNV_REQUIRE(rows >= 0 && rows < (1LL << 31) - 256, "bad row count");
+  PNV_REQUIRE(features >= 1 && k >= 1, "features and k must be positive");
+  PNV_REQUIRE(features < (1 << 30) && k < (1 << 29), "features or k too large");
+  LinearArgs a{};
+  if (gated) {
+    PNV_REQUIRE(act_kind == PNV_ACT_SILU || act_kind == PNV_ACT_SITU, "activation must be 'silu' or 'situ' when gated, got kind %d", act_kind);
+    if (int rc = make_gated_act(act_kind, beta, linear_beta, a.act)) return rc;
+    PNV_REQUIRE(features % 64 == 0, "gated: features (gates and ups in 64-row blocks) must be a multiple of 64, got %d", features);
+  } else {
+    PNV_REQUIRE(act_kind == PNV_ACT_NONE || act_kind == PNV_ACT_RELU || act_kind == PNV_ACT_SILU || act_kind == PNV_ACT_GELU,
+                "activation must be 'none', 'relu', 'silu' or 'gelu' unless gated, got kind %d", act_kind);
+  }
+  const int n_out = gated ? features / 2 : features;
+  if (mx8) PNV_REQUIRE(k % kSfBlock == 0, "K must be a multiple of %d, got %d", kSfBlock, k);
+  else PNV_REQUIRE(k % 8 == 0, "K must be a multiple of 8, got %d", k);
+  if (rows == 0) return PNV_OK;
+  PNV_REQUIRE(out && x && w && (!mx8 || (x_sf && w_sf)), "null pointer argument");
+  const long long k_bytes = mx8 ? k : 2LL * k, stride_bytes = mx8 ? x_stride : 2 * x_stride;
+  PNV_REQUIRE(x_stride >= k && stride_bytes % 16 == 0, "rows of x must not overlap and start at multiples of 16 bytes");
+  PNV_REQUIRE(at(x, 16) && at(w, 16), "the operands must be 16-byte aligned");
+  PNV_REQUIRE(!mx8 || (at(x_sf, 16) && at(w_sf, 16)), "the scales must be 16-byte aligned");
+  PNV_REQUIRE(at(out, out_is_f32 ? 4 : 2) && at(bias, bias_is_f32 ? 4 : 2) && at(residual, 2), "a buffer is not aligned to its elements");
+  PNV_REQUIRE(residual == nullptr || residual_stride >= n_out, "rows of the residual must not overlap");
+  a.out = out;
+  a.bias = bias;
+  a.residual = static_cast<const __nv_bfloat16*>(residual);
+  a.x_sf = x_sf;
+  a.w_sf = w_sf;
+  a.residual_stride = residual_stride;
+  a.rows = (int)rows;
+  a.features = features;
+  a.n_out = n_out;
+  a.k_bytes = (int)k_bytes;
+  a.out_f32 = out_is_f32;
+  a.bias_f32 = bias_is_f32;
+  a.gated = gated;
+  a.kind = act_kind;
+  // (pieces of a row start at multiples of 8 outputs, those of the pair kernel at multiples of 16)
+  const int out_pitch = n_out * (out_is_f32 ? 4 : 2);
+  a.vec_out = out_pitch % 32 == 0 && at(out, 32) ? 32 : out_pitch % 16 == 0 && at(out, 16) ? 16 : 0;
+  a.vec_residual = residual_stride % 8 == 0 && at(residual, 16) ? 16 : 0;
+  a.vec_bias = at(bias, 16) ? 16 : 0;
+  if (sm_count <= 0) sm_count = 148;
+  const Operands o{x, w, stride_bytes};
+  return mx8 ? run_linear<true>(o, a, sm_count, stream) : run_linear<false>(o, a, sm_count, stream);
+}
+
+}  // namespace
+}  // namespace pnv
+
+using namespace pnv;
+
+extern "C" int pnv_linear(void* out, int out_is_f32, const void* x, int64_t x_stride, const void* w, const void* bias, int bias_is_f32,
+                          const void* residual, int64_t residual_stride, int64_t rows, int features, int k, int act_kind, int gated,
+                          float beta, float linear_beta, int sm_count, pnv_stream_t stream) {
+  return linear_common(false, out, out_is_f32, x, x_stride, nullptr, w, nullptr, bias, bias_is_f32, residual, residual_stride, rows,
+                       features, k, act_kind, gated, beta, linear_beta, sm_count, (cudaStream_t)stream);
+}
+
+extern "C" int pnv_linear_mx8(void* out, const uint8_t* x, const uint8_t* x_sf, const uint8_t* w, const uint8_t* w_sf, const void* bias,
+                              int bias_is_f32, const void* residual, int64_t residual_stride, int64_t rows, int features, int k,
+                              int act_kind, int gated, float beta, float linear_beta, int sm_count, pnv_stream_t stream) {
+  return linear_common(true, out, 0, x, k, x_sf, w, w_sf, bias, bias_is_f32, residual, residual_stride, rows, features, k, act_kind, gated,
+                       beta, linear_beta, sm_count, (cudaStream_t)stream);
+}
+
+extern "C" int pnv_linear_device_status(int* status_out) {
+  PNV_REQUIRE(status_out, "null pointer argument");
+  PNV_CUDA(cudaDeviceSynchronize());
+  PNV_CUDA(cudaMemcpyFromSymbol(status_out, g_linear_status, sizeof(int)));
+  int zero = 0;
+  PNV_CUDA(cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(int)));
+  return PNV_OK;
+}

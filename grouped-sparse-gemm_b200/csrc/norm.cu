@@ -1,0 +1,289 @@
+// The root-mean-square norm ahead of a block, with the residual's addition, and the 8-bit quantizer of the dense products.
+//
+//   v = x + residual;  n = v / sqrt(mean(v^2) + eps) * weight        (all in 32 bits)
+//   residual_out = bf16(v), y = bf16(n), (q, q_sf) = 8-bit codes of n
+// Codes and y are both rounded from n itself: codes made of the rounded y would carry two roundings.
+//
+// The 8-bit format: e4m3 codes with one e8m0 scale (a power of two, byte b stands for 2^(b - 127)) per 32 elements, the
+// smallest that leaves the block's largest magnitude at 448 or below, so that no element saturates; a block of zeros has
+// scale 1, a block that holds an infinity or a NaN scale byte 0xFF (NaN) and NaN codes.  Scales lie in the same 512-byte
+// atoms as the grouped GEMM's (common.cuh), slop filled with 1.0: a product multiplies what it finds there by zeros.
+#include "common.cuh"
+#include "mx8.cuh"
+
+namespace pnv {
+namespace {
+
+constexpr int kVecElems = 8;             // elements a lane holds of each of its pieces: 16 bytes of bf16
+
+struct NormArgs {
+  const __nv_bfloat16* x;
+  const __nv_bfloat16* residual;         // or nullptr
+  const void* weight;
+  __nv_bfloat16* y;                      // or nullptr
+  __nv_bfloat16* residual_out;
+  uint8_t* q;                            // or nullptr
+  uint8_t* q_sf;
+  long long x_stride, residual_stride;
+  long long rows, padded_rows;           // rows up to padded_rows only have scales, of slop
+  int width, weight_f32;
+  int team;                              // threads per row, a multiple of 32; a block has one row where it is above 32
+  float eps;
+};
+
+// Eight neighbouring elements; kVec: as one 16-byte load, else one by one and zeros from `width` on.
+template <bool kVec>
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int i, int width) {
+  if constexpr (kVec) {
+    return __ldg(reinterpret_cast<const uint4*>(row) + i);
+  } else {
+    uint32_t h[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      h[j] = i * 8 + j < width ? __ldg(reinterpret_cast<const unsigned short*>(row) + i * 8 + j) : 0u;
+    return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+  }
+}
+template <bool kVec>
+__device__ __forceinline__ void store8(__nv_bfloat16* row, int i, int width, const float (&f)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = as_u32(__floats2bfloat162_rn(f[2 * j], f[2 * j + 1]));
+  if constexpr (kVec) {
+    reinterpret_cast<uint4*>(row)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i * 8 + j < width)
+        reinterpret_cast<unsigned short*>(row)[i * 8 + j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
+  }
+}
+template <bool kVec>
+__device__ __forceinline__ void load_weight8(const void* weight, int f32, int i, int width, float (&w)[8]) {
+  if (!f32) {
+    unpack8(load8<kVec>(static_cast<const __nv_bfloat16*>(weight), i, width), w);
+  } else if (kVec) {
+    const float4 a = __ldg(static_cast<const float4*>(weight) + 2 * i), b = __ldg(static_cast<const float4*>(weight) + 2 * i + 1);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = i * 8 + j < width ? __ldg(static_cast<const float*>(weight) + i * 8 + j) : 0.f;
+  }
+}
+
+// A team of `team` threads takes a row and keeps all of it in registers, V pieces of eight elements a thread, so that
+// memory is read once.  Bound: HBM (9 bytes and 1/32 per element with both outputs).
+template <int V, bool kVec>
+__global__ void __launch_bounds__(512)
+add_rms_norm_kernel(const NormArgs a) {
+  __shared__ float s_sum[16];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x % a.team, per_block = blockDim.x / a.team;
+  const long long row = (long long)blockIdx.x * per_block + threadIdx.x / a.team;
+  const int n_kt = (a.width + 127) / 128;
+  uint8_t* sf_row = a.q_sf + ((row >> 7) * n_kt) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+  if (row >= a.rows) {                   // (whole teams, so whole warps; with team > 32 the whole block)
+    if (a.q != nullptr && row < a.padded_rows)
+      for (int i = lane; i < n_kt; i += a.team) *reinterpret_cast<uint32_t*>(sf_row + i * 512LL) = kMx8SlopWord;
+    return;
+  }
+  const int n = (a.width + kVecElems - 1) / kVecElems;
+  const __nv_bfloat16* x = a.x + row * a.x_stride;
+  float v[V][8];
+  float sum = 0.f;
+  {
+    uint4 raw[V];
+#pragma unroll
+    for (int p = 0; p < V; ++p) {
+      const int i = p * a.team + lane;
+      raw[p] = i < n ? load8<kVec>(x, i, a.width) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (a.residual != nullptr) {
+      const __nv_bfloat16* r = a.residual + row * a.residual_stride;
+      uint4 more[V];
+#pragma unroll
+      for (int p = 0; p < V; ++p) {
+        const int i = p * a.team + lane;
+        more[p] = i < n ? load8<kVec>(r, i, a.width) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int p = 0; p < V; ++p) {
+        const int i = p * a.team + lane;
+        float f[8];
+        unpack8(raw[p], v[p]);
+        unpack8(more[p], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[p][j] += f[j];
+        if (i < n) store8<kVec>(a.residual_out + row * a.width, i, a.width, v[p]);
+      }
+    } else {
+#pragma unroll
+      for (int p = 0; p < V; ++p) unpack8(raw[p], v[p]);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < V; ++p)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = fmaf(v[p][j], v[p][j], sum);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (a.team > 32) {
+    if ((lane & 31) == 0) s_sum[lane >> 5] = sum;
+    __syncthreads();
+    sum = 0.f;
+    for (int w = 0; w < a.team / 32; ++w) sum += s_sum[w];
+  }
+  const float rstd = __frsqrt_rn(__fdiv_rn(sum, (float)a.width) + a.eps);
+#pragma unroll
+  for (int p = 0; p < V; ++p) {
+    const int i = p * a.team + lane;
+    if (i < n) {
+      float w[8];
+      load_weight8<kVec>(a.weight, a.weight_f32, i, a.width, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[p][j] = __fmul_rn(__fmul_rn(v[p][j], rstd), w[j]);
+      if (a.y != nullptr) store8<kVec>(a.y + row * a.width, i, a.width, v[p]);
+    }
+    if (a.q != nullptr) {                // four lanes hold a block, sixteen the four blocks of a word of scales
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[p][j]) & 0x7FFFFFFFu);
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const uint32_t byte = i < n ? mx8_scale_byte(m) : kMx8One;
+      if (i < n) {
+        const float inv = mx8_inverse(byte);
+        reinterpret_cast<uint2*>(a.q + row * a.width)[i] = make_uint2(mx8_codes4(v[p], 0, byte, inv), mx8_codes4(v[p], 4, byte, inv));
+      }
+      uint32_t word = byte << (8 * ((lane >> 2) & 3));
+      word |= __shfl_xor_sync(0xffffffffu, word, 4);
+      word |= __shfl_xor_sync(0xffffffffu, word, 8);
+      if ((lane & 15) == 0 && (i >> 4) < n_kt) *reinterpret_cast<uint32_t*>(sf_row + (i >> 4) * 512LL) = word;
+    }
+  }
+}
+
+constexpr int kQuantThreads = 256;
+
+// A lane takes a block of 32 elements, four lanes the blocks of one word of scales ("quad": 128 elements of a row).  Quads
+// of all rows are laid end to end, rows padded to whole atoms among them: their scales are written here too.
+__global__ void __launch_bounds__(kQuantThreads)
+quant_mx8_kernel(const __nv_bfloat16* __restrict__ x, long long x_stride, unsigned rows, unsigned quads, int K, int n_kt,
+                 uint8_t* __restrict__ q, uint8_t* __restrict__ q_sf) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const unsigned quad = blockIdx.x * (kQuantThreads / 4) + threadIdx.x / 4;
+  const unsigned row = quad / (unsigned)n_kt;
+  const int atom = (int)(quad - row * (unsigned)n_kt), part = threadIdx.x & 3;
+  const int kb = atom * 4 + part;
+  uint32_t byte = kMx8One;
+  if (quad < quads && row < rows && kb < K / kSfBlock) {
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(x + row * x_stride) + kb * 64LL;
+    uint32_t w[16];
+    if (((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(x_stride * 2)) & 31) == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+            : "=r"(w[8 * h]), "=r"(w[8 * h + 1]), "=r"(w[8 * h + 2]), "=r"(w[8 * h + 3]), "=r"(w[8 * h + 4]), "=r"(w[8 * h + 5]),
+              "=r"(w[8 * h + 6]), "=r"(w[8 * h + 7]) : "l"(src + 32 * h) : "memory");
+    } else {
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const uint4 t = __ldg(reinterpret_cast<const uint4*>(src) + h);
+        w[4 * h] = t.x; w[4 * h + 1] = t.y; w[4 * h + 2] = t.z; w[4 * h + 3] = t.w;
+      }
+    }
+    uint32_t m = 0;                      // magnitudes of bf16 numbers order like their bits, infinities and NaNs above all
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    byte = mx8_scale_byte(max(m & 0xFFFFu, m >> 16) << 16);
+    const float inv = mx8_inverse(byte);
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f[4] = {bf16_lo(w[2 * i]), bf16_hi(w[2 * i]), bf16_lo(w[2 * i + 1]), bf16_hi(w[2 * i + 1])};
+      c[i] = mx8_codes4(f, 0, byte, inv);
+    }
+    uint4* dst = reinterpret_cast<uint4*>(q + (long long)row * K + kb * 32LL);
+    dst[0] = make_uint4(c[0], c[1], c[2], c[3]);
+    dst[1] = make_uint4(c[4], c[5], c[6], c[7]);
+  }
+  uint32_t word = byte << (8 * part);
+  word |= __shfl_xor_sync(0xffffffffu, word, 1);
+  word |= __shfl_xor_sync(0xffffffffu, word, 2);
+  if (part == 0 && quad < quads)
+    *reinterpret_cast<uint32_t*>(q_sf + ((long long)(row >> 7) * n_kt + atom) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4) = word;
+}
+
+template <int V>
+cudaError_t launch_norm(const NormArgs& a, bool vec, dim3 grid, dim3 block, cudaStream_t s) {
+  return launch_pdl(vec ? add_rms_norm_kernel<V, true> : add_rms_norm_kernel<V, false>, grid, block, 0, s, pdl_enabled(), a);
+}
+
+bool aligned_to(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+}  // namespace
+}  // namespace pnv
+
+using namespace pnv;
+
+extern "C" int pnv_add_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
+                                int weight_is_f32, float eps, int64_t rows, int width, void* y, void* residual_out, uint8_t* q,
+                                uint8_t* q_sf, int sm_count, pnv_stream_t stream) {
+  PNV_REQUIRE(rows >= 0 && rows < (1LL << 31), "bad row count");
+  PNV_REQUIRE(width >= 1 && width <= PNV_NORM_MAX_WIDTH, "add_rms_norm: rows of 1 to %d elements, got %d", PNV_NORM_MAX_WIDTH, width);
+  PNV_REQUIRE(y != nullptr || q != nullptr, "add_rms_norm: at least one of y and q is written");
+  PNV_REQUIRE((q == nullptr) == (q_sf == nullptr), "null pointer argument");
+  PNV_REQUIRE(q == nullptr || width % kSfBlock == 0, "8-bit output: the width must be a multiple of %d, got %d", kSfBlock, width);
+  PNV_REQUIRE(eps >= 0.f, "eps must not be negative");
+  if (rows == 0) return PNV_OK;
+  PNV_REQUIRE(x && weight && (residual == nullptr) == (residual_out == nullptr), "null pointer argument");
+  PNV_REQUIRE(x_stride >= width && (residual == nullptr || residual_stride >= width), "rows must not overlap");
+  PNV_REQUIRE(aligned_to(x, 2) && aligned_to(residual, 2) && aligned_to(weight, weight_is_f32 ? 4 : 2) && aligned_to(y, 2) &&
+                  aligned_to(residual_out, 2) && aligned_to(q, 8) && aligned_to(q_sf, 4),
+              "add_rms_norm: a buffer is not aligned to its elements (codes 8 bytes, scales 4)");
+  const bool vec = width % 8 == 0 && x_stride % 8 == 0 && residual_stride % 8 == 0 && aligned_to(x, 16) && aligned_to(residual, 16) &&
+                   aligned_to(weight, 16) && aligned_to(y, 16) && aligned_to(residual_out, 16);
+  const int n = ceil_div_i(width, kVecElems);
+  if (sm_count <= 0) sm_count = 148;
+  // Many rows: as few threads a row as hold it with eight pieces each.  Rows that leave SMs without work: two pieces each
+  // (up to 512 threads), so that a row takes as little time as it can.
+  int team = 32;
+  while (team < 512 && ceil_div_i(n, team) > (rows <= 2LL * sm_count ? 2 : 8)) team *= 2;
+  const int threads = team > 32 ? team : 128;
+  NormArgs a{(const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, weight, (__nv_bfloat16*)y, (__nv_bfloat16*)residual_out, q, q_sf,
+             x_stride, residual_stride, rows, q ? (rows + 127) / 128 * 128 : rows, width, weight_is_f32, team, eps};
+  const long long blocks = (a.padded_rows + threads / team - 1) / (threads / team);
+  const dim3 grid((unsigned)blocks), block((unsigned)threads);
+  cudaStream_t s = (cudaStream_t)stream;
+  switch (ceil_div_i(n, team)) {
+    case 1: PNV_CUDA(launch_norm<1>(a, vec, grid, block, s)); break;
+    case 2: PNV_CUDA(launch_norm<2>(a, vec, grid, block, s)); break;
+    case 3: PNV_CUDA(launch_norm<3>(a, vec, grid, block, s)); break;
+    case 4: PNV_CUDA(launch_norm<4>(a, vec, grid, block, s)); break;
+    case 5: PNV_CUDA(launch_norm<5>(a, vec, grid, block, s)); break;
+    case 6: PNV_CUDA(launch_norm<6>(a, vec, grid, block, s)); break;
+    case 7: PNV_CUDA(launch_norm<7>(a, vec, grid, block, s)); break;
+    default: PNV_CUDA(launch_norm<8>(a, vec, grid, block, s)); break;
+  }
+  return PNV_OK;
+}
+
+extern "C" int pnv_quant_mx8(const void* x, int64_t x_stride, int64_t rows, int k, uint8_t* q, uint8_t* q_sf, pnv_stream_t stream) {
+  PNV_REQUIRE(k > 0 && k % kSfBlock == 0, "K must be a multiple of %d, got %d", kSfBlock, k);
+  PNV_REQUIRE(rows >= 0 && rows < (1LL << 31), "bad row count");
+  if (rows == 0) return PNV_OK;
+  PNV_REQUIRE(x && q && q_sf, "null pointer argument");
+  PNV_REQUIRE(x_stride >= k && x_stride % 8 == 0, "rows must not overlap and start at multiples of 16 bytes");
+  PNV_REQUIRE(aligned_to(x, 16) && aligned_to(q, 16) && aligned_to(q_sf, 4),
+              "quant_mx8: the bf16 rows and the codes must be 16-byte aligned, the scales 4-byte");
+  const int n_kt = sf_k_atoms(k);
+  const long long quads = (rows + 127) / 128 * 128 * n_kt;
+  PNV_REQUIRE(quads < (1LL << 32) - kQuantThreads, "too many rows");
+  PNV_CUDA(launch_pdl(quant_mx8_kernel, dim3((unsigned)((quads + kQuantThreads / 4 - 1) / (kQuantThreads / 4))), dim3(kQuantThreads), 0,
+                      (cudaStream_t)stream, pdl_enabled(), (const __nv_bfloat16*)x, (long long)x_stride, (unsigned)rows, (unsigned)quads, k,
+                      n_kt, q, q_sf));
+  return PNV_OK;
+}

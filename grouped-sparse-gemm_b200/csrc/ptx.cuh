@@ -121,6 +121,15 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint64_t* bar, uint32_t cta)
       : "memory");
 }
 
+// Four floats at the address that `p` (shared memory of this CTA) has in CTA `cta` of this cluster.
+__device__ __forceinline__ float4 ld_cluster_f4(const float* p, uint32_t cta) {
+  float4 v;
+  asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %4, %5;\n\t"
+               "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n\t}"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_u32(p)), "r"(cta) : "memory");
+  return v;
+}
+
 // ---- TMA -----------------------------------------------------------------------------------------
 
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* m) {
@@ -333,6 +342,45 @@ __host__ __device__ constexpr uint32_t mma_sp_nvf4_idesc(int n, int m = 128) {
   return (1u << 2) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// Dense products, K-major operands, fp32 accumulation in tensor memory.  CTAS = 2 as above: 256 rows of A (128 from each
+// CTA), N rows of B (half from each).
+//
+// D (+)= A * B^T, bf16 operands, 16 K (32 bytes) per instruction.
+template <int CTAS = 1>
+__device__ __forceinline__ void tc_mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  if (CTAS == 2)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// D format (fp32 = 1) bits 4-5, A / B format (bf16 = 1) bits 7-9 / 10-12, N/8 bits 17-22, M/16 bits 24-28.
+__host__ __device__ constexpr uint32_t mma_bf16_idesc(int n, int m) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// The same for e4m3 operands with one e8m0 scale per row and 32 K, 32 K (32 bytes) per instruction.  A scale word in tensor
+// memory holds the bytes of four K-blocks; the instruction descriptor says which of them is meant.
+template <int CTAS = 1>
+__device__ __forceinline__ void tc_mma_mxf8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate,
+                                            uint32_t sfa_tmem, uint32_t sfb_tmem) {
+  if (CTAS == 2)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+                 :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+                 :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem) : "memory");
+}
+// A / B format (e4m3 = 0), scale byte of B bits 4-5, N/8 bits 17-22, scale format (1 = UE8M0) bit 23, M/16 bits 24-28, scale
+// byte of A bits 29-30.
+__host__ __device__ constexpr uint32_t mma_mxf8_idesc(int n, int m, int scale_byte) {
+  return ((uint32_t)scale_byte << 4) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) | ((uint32_t)scale_byte << 29);
+}
+
 // The matrix-fragment form: 16 lanes x 8 columns per step (16x256b), 4 or 2 steps.  Of step j a thread gets
 // r[4j], r[4j+1] = (lane l / 4, columns 8j + 2 (l % 4) and the next one) and r[4j+2], r[4j+3] = the same columns eight
 // lanes further on: two neighbouring columns of a row packed to 16 bits are an 8 x 8 fragment stmatrix can transpose.
@@ -369,6 +417,16 @@ __device__ __forceinline__ void tc_ld_32x32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
         "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
         "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// the same for 16 columns
+__device__ __forceinline__ void tc_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
 }

@@ -1,0 +1,253 @@
+// Router logits to the top-k experts and weights that dispatch_plan and moe_finalize take.
+//
+//   score = softmax or sigmoid of the logits; experts are ranked by score + bias, or by the logit where there is no bias (the
+//   scores rise with it), groups of neighbouring experts by the sum of their two best keys (their best one without a bias),
+//   ties going to the lowest index; the weights are the scores of the chosen, over their sum if asked for, times a factor.
+//
+// A warp takes a token: its keys lie in registers as unsigned numbers that order like them, every round of the selection is
+// two warp-wide integer reductions (largest key, lowest expert that has it).  Keys with a bias are sums of 32-bit roundings,
+// so two that lie closer together than those can be off might come out in the wrong order: where a selected key is that
+// close to the next one, the row is done again in 64 bits (a handful of rows in a thousand at 256 experts).
+// Bound: latency of the reductions for few rows, issue slots for many.
+#include <climits>
+
+#include "common.cuh"
+
+namespace pnv {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr unsigned kAll = 0xffffffffu;
+
+struct RouteArgs {
+  const void* logits;
+  const float* bias;             // or nullptr
+  float* weights;
+  int* ids;
+  long long rows, stride;
+  int experts, topk, groups, topk_groups, group_size;
+  unsigned group_inv;            // ceil(2^20 / group_size)
+  int bf16, sigmoid, renormalize;
+  float scale;
+};
+
+__device__ __forceinline__ float logit_at(const RouteArgs& a, const void* row, int e) {
+  return a.bf16 ? __uint_as_float((uint32_t)__ldg(static_cast<const unsigned short*>(row) + e) << 16)
+                : __ldg(static_cast<const float*>(row) + e);
+}
+
+// Unsigned numbers that order like the keys; 0 stands for an expert that cannot be chosen, 1 for a NaN.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t b = __float_as_uint(v + 0.f);                         // (-0 counts as 0)
+  if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 1u;
+  return (b >> 31) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ unsigned long long order_of(double v) {
+  const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
+  if ((b & 0x7FFFFFFFFFFFFFFFull) > 0x7FF0000000000000ull) return 1ull;
+  return (b >> 63) ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ float key_of(uint32_t o) { return o == 1u ? -INFINITY : __uint_as_float((o >> 31) ? o & 0x7FFFFFFFu : ~o); }
+__device__ __forceinline__ double key_of(unsigned long long o) {
+  return o == 1ull ? -INFINITY : __longlong_as_double((long long)((o >> 63) ? o & 0x7FFFFFFFFFFFFFFFull : ~o));
+}
+
+__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(kAll, v); }
+__device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
+  const uint32_t hi = __reduce_max_sync(kAll, (uint32_t)(v >> 32));
+  const uint32_t lo = __reduce_max_sync(kAll, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+  return (unsigned long long)hi << 32 | lo;
+}
+
+__device__ __forceinline__ float sigmoid_of(float l) { return rcp_approx(1.f + ex2_approx(l * -kLog2e)); }
+__device__ __forceinline__ double sigmoid_of(double l) { return 1.0 / (1.0 + exp(-l)); }
+__device__ __forceinline__ float exp_of(float v) { return expf(v); }
+__device__ __forceinline__ double exp_of(double v) { return exp(v); }
+
+// exp(l - mx), 1 where the two are the same infinity, 0 everywhere in a row of nothing but -infinity.
+template <class F>
+__device__ __forceinline__ F softmax_part(F l, F mx) { return mx == (F)-INFINITY ? (F)0 : l == mx ? (F)1 : exp_of(l - mx); }
+
+__device__ __forceinline__ float row_max(const RouteArgs& a, const void* row, int lane) {
+  uint32_t m = 0;
+  for (int e = lane; e < a.experts; e += 32) m = max(m, order_of(logit_at(a, row, e)));
+  m = warp_max(m);
+  return m == 1u ? -INFINITY : key_of(m);
+}
+template <class F>
+__device__ __forceinline__ F softmax_sum(const RouteArgs& a, const void* row, int lane, F mx) {
+  F sum = 0;
+  for (int e = lane; e < a.experts; e += 32) sum += softmax_part((F)logit_at(a, row, e), mx);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+  return sum;
+}
+
+// Are two neighbouring keys, the larger one first, too close for 32 bits to order?  A score is off by at most 1.5e-6 (a softmax over 1024), its sum
+// with the bias by half a unit more; a group's sum of two by twice that.
+__device__ __forceinline__ bool too_close(float larger, float smaller, float terms) {
+  return larger - smaller <= terms * 3.8146973e-6f * (1.f + fabsf(larger));
+}
+
+// Lane r < topk returns expert r of the row, best first.  doubtful: (32 bits with a bias) the order is not certain.
+template <class F, class O, int VPL>
+__device__ __forceinline__ int select(const RouteArgs& a, const void* row, int lane, bool& doubtful) {
+  const bool check = sizeof(F) == 4 && a.bias != nullptr;
+  O key[VPL];
+  {
+    F mx = 0, total = 1;
+    if (a.bias != nullptr && !a.sigmoid) {
+      mx = (F)row_max(a, row, lane);
+      total = softmax_sum<F>(a, row, lane, mx);
+    }
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      const int e = j * 32 + lane;
+      key[j] = 0;
+      if (e < a.experts) {
+        F k = (F)logit_at(a, row, e);
+        if (a.bias != nullptr) k = (a.sigmoid ? sigmoid_of(k) : softmax_part(k, mx) / total) + (F)__ldg(a.bias + e);
+        key[j] = order_of(k);
+      }
+    }
+  }
+  doubtful = false;
+  if (a.groups > 1) {
+    O mine = 0;                          // lane g: the score of group g
+    for (int g = 0; g < a.groups; ++g) {
+      O first = 0, second = 0;           // this lane's two best of the group
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        const bool in = (((unsigned)(j * 32 + lane) * a.group_inv) >> 20) == (unsigned)g;
+        const O k = in ? key[j] : (O)0;
+        second = max(second, min(first, k));
+        first = max(first, k);
+      }
+      const O best = warp_max(first);
+      O score = best;
+      if (a.bias != nullptr) {
+        const int owner = __ffs(__ballot_sync(kAll, first == best)) - 1;
+        const O next = warp_max(lane == owner ? second : first);
+        score = next == 0 ? best : order_of(key_of(best) + key_of(next));
+      }
+      if (lane == g) mine = score;
+    }
+    unsigned kept = 0;
+    F last = 0;
+    for (int r = 0; r <= a.topk_groups && r < a.groups; ++r) {
+      const O best = warp_max(mine);
+      const int g = __ffs(__ballot_sync(kAll, mine == best && lane < a.groups)) - 1;
+      const F k = key_of(best);
+      // (the order among the kept does not matter, only the border)
+      if (r == a.topk_groups) {
+        if (check) doubtful |= too_close((float)last, (float)k, 2.f);
+        break;
+      }
+      last = k;
+      kept |= 1u << g;
+      if (lane == g) mine = 0;
+    }
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      const unsigned g = ((unsigned)(j * 32 + lane) * a.group_inv) >> 20;
+      if (g >= 32 || !((kept >> g) & 1)) key[j] = 0;
+    }
+  }
+  int picked = 0;
+  F last = 0;
+  const int rounds = check ? a.topk + 1 : a.topk;         // one more to see how close the next one is
+  for (int r = 0; r < rounds; ++r) {
+    O first = key[0];
+#pragma unroll
+    for (int j = 1; j < VPL; ++j) first = max(first, key[j]);
+    const O best = warp_max(first);
+    if (best == 0) break;                // (only the round beyond the last: there are topk experts to choose from)
+    int e = INT_MAX;
+#pragma unroll
+    for (int j = VPL - 1; j >= 0; --j)
+      if (key[j] == best) e = j * 32 + lane;
+    e = __reduce_min_sync(kAll, e);
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+      if (e == j * 32 + lane) key[j] = 0;
+    if (check) {
+      const F k = key_of(best);
+      if (r > 0) doubtful |= too_close((float)last, (float)k, 1.f);
+      last = k;
+    }
+    if (lane == r) picked = e;
+  }
+  return picked;
+}
+
+template <int VPL>
+__device__ __noinline__ int select_exactly(const RouteArgs& a, const void* row, int lane) {
+  bool ignored;
+  return select<double, unsigned long long, VPL>(a, row, lane, ignored);
+}
+
+template <int VPL>
+__global__ void __launch_bounds__(kWarps * 32)
+route_topk_kernel(const RouteArgs a) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const long long t = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (t >= a.rows) return;
+  const void* row = static_cast<const uint8_t*>(a.logits) + t * a.stride * (a.bf16 ? 2 : 4);
+  bool doubtful;
+  int e = select<float, uint32_t, VPL>(a, row, lane, doubtful);
+  if (doubtful) e = select_exactly<VPL>(a, row, lane);
+  float w = 0.f;
+  if (a.sigmoid) {
+    if (lane < a.topk) w = __fdiv_rn(1.f, 1.f + expf(-logit_at(a, row, e)));
+  } else {
+    const float mx = row_max(a, row, lane);
+    if (lane < a.topk) w = softmax_part(logit_at(a, row, e), mx);
+    if (!a.renormalize) {
+      const float total = softmax_sum<float>(a, row, lane, mx);
+      w = total > 0.f ? __fdiv_rn(w, total) : total;               // (a NaN stays one)
+    }
+  }
+  if (a.renormalize) {
+    float sum = w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+    w = sum == 0.f ? 0.f : __fdiv_rn(w, sum);
+  }
+  if (lane < a.topk) {
+    a.ids[t * a.topk + lane] = e;
+    a.weights[t * a.topk + lane] = w * a.scale;
+  }
+}
+
+}  // namespace
+}  // namespace pnv
+
+using namespace pnv;
+
+extern "C" int pnv_route_topk(const void* logits, int logits_are_bf16, int64_t stride, int64_t rows, int experts, int topk, int sigmoid,
+                              const float* bias, int groups, int topk_groups, int renormalize, float scale, float* weights,
+                              int32_t* ids, pnv_stream_t stream) {
+  PNV_REQUIRE(rows >= 0 && rows < (1LL << 31), "bad row count");
+  PNV_REQUIRE(experts >= 1 && experts <= PNV_ROUTE_MAX_EXPERTS, "route_topk: 1 to %d experts, got %d", PNV_ROUTE_MAX_EXPERTS, experts);
+  PNV_REQUIRE(groups >= 1 && groups <= 32 && experts % groups == 0, "groups must divide the experts, at most 32, got %d", groups);
+  PNV_REQUIRE(topk_groups >= 1 && topk_groups <= groups, "topk_groups must be in [1, groups], got %d", topk_groups);
+  PNV_REQUIRE(topk >= 1 && topk <= 32 && topk <= experts / groups * topk_groups,
+              "topk must be in [1, 32] and leave every choice an expert, got %d of %d", topk, experts / groups * topk_groups);
+  if (rows == 0) return PNV_OK;
+  PNV_REQUIRE(logits && weights && ids, "null pointer argument");
+  PNV_REQUIRE(stride >= experts, "rows must not overlap");
+  PNV_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (logits_are_bf16 ? 2 : 4) == 0 && reinterpret_cast<uintptr_t>(bias) % 4 == 0 &&
+                  reinterpret_cast<uintptr_t>(weights) % 4 == 0 && reinterpret_cast<uintptr_t>(ids) % 4 == 0,
+              "route_topk: a buffer is not aligned to its elements");
+  const int group_size = experts / groups;
+  // (e * ceil(2^20 / size)) >> 20 is e / size for e below 1024: the product is off by less than e / 2^20 < 1 / size)
+  RouteArgs a{logits, bias, weights, (int*)ids, rows, stride, experts, topk, groups, topk_groups, group_size,
+              (unsigned)(((1 << 20) + group_size - 1) / group_size), logits_are_bf16, sigmoid, renormalize, scale};
+  const int vpl = ceil_div_i(experts, 32);
+  auto kernel = vpl <= 1 ? route_topk_kernel<1> : vpl <= 2 ? route_topk_kernel<2> : vpl <= 4 ? route_topk_kernel<4>
+              : vpl <= 8 ? route_topk_kernel<8> : vpl <= 16 ? route_topk_kernel<16> : route_topk_kernel<32>;
+  PNV_CUDA(launch_pdl(kernel, dim3((unsigned)((rows + kWarps - 1) / kWarps)), dim3(kWarps * 32), 0, (cudaStream_t)stream, pdl_enabled(), a));
+  return PNV_OK;
+}

@@ -633,6 +633,168 @@ std::tuple<Tensor, Tensor> group_mm_swiglu_quant(const Tensor& a_comp, const Ten
   return {b_out, sfb_out};
 }
 
+// ---- around the grouped GEMM: norm, 8-bit quantizer, dense layers, routing (no counterpart in the reference) ------------
+
+// Rows of a 2-D bf16 tensor may lie apart (a slice of wider rows), their elements may not.
+void check_rows(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.dim() == 2 && is_bf16(t) && (t.size(1) <= 1 || t.stride(1) == 1), what);
+}
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max<int64_t>(t.size(1), 1); }
+
+void check_same_device(const Tensor& t, const Tensor& like, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), what, " must be on the device of the first operand");
+}
+
+int check_bias(const optional<Tensor>& bias, const Tensor& like, int64_t n, const char* what) {
+  if (!bias.has_value()) return 0;
+  check_same_device(*bias, like, what);
+  TORCH_CHECK((is_bf16(*bias) || is_float(*bias)) && bias->is_contiguous() && bias->dim() == 1 && bias->numel() == n, what,
+              " must be contiguous bf16 or float32 [", n, "]");
+  return is_float(*bias) ? 1 : 0;
+}
+
+// (y, residual_out, q, q_sf); what was not asked for is empty
+std::tuple<Tensor, Tensor, Tensor, Tensor> add_rms_norm(const Tensor& x, const optional<Tensor>& residual, const Tensor& weight, double eps,
+                                                        bool out_bf16, bool out_mx8) {
+  TORCH_CHECK(x.is_cuda() && weight.is_cuda(), "inputs must be CUDA tensors");
+  check_arch(x);
+  check_rows(x, "x must be bf16 [T, hidden] with contiguous rows");
+  const int64_t T = x.size(0), H = x.size(1);
+  TORCH_CHECK(H >= 1 && H <= PNV_NORM_MAX_WIDTH, "hidden must be in [1, ", PNV_NORM_MAX_WIDTH, "], got ", H);
+  check_bias(weight, x, H, "weight");
+  TORCH_CHECK(eps >= 0, "eps must not be negative");
+  TORCH_CHECK(out_bf16 || out_mx8, "at least one of out_bf16 and out_mx8 must be set");
+  TORCH_CHECK(!out_mx8 || H % kSfBlock == 0, "hidden must be a multiple of ", kSfBlock, " for 8-bit output, got ", H);
+  if (residual.has_value()) {
+    check_same_device(*residual, x, "residual");
+    check_rows(*residual, "residual must be bf16 [T, hidden] with contiguous rows");
+    TORCH_CHECK(residual->size(0) == T && residual->size(1) == H, "residual must be shaped like x");
+  }
+  Tensor y = empty_on(x, {out_bf16 ? T : 0, H}, at::kBFloat16);
+  Tensor r = empty_on(x, {residual.has_value() ? T : 0, H}, at::kBFloat16);
+  Tensor q = empty_on(x, {out_mx8 ? T : 0, H}, at::kFloat8_e4m3fn);
+  Tensor q_sf = empty_on(x, {out_mx8 ? pnv_sf_numel((int)T, (int)H, 1) : 0}, at::kFloat8_e8m0fnu);
+  if (T == 0) return {y, r, q, q_sf};
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_rc(pnv_add_rms_norm(x.const_data_ptr(), row_stride(x), residual.has_value() ? residual->const_data_ptr() : nullptr,
+                            residual.has_value() ? row_stride(*residual) : 0, weight.const_data_ptr(), is_float(weight) ? 1 : 0, (float)eps, T,
+                            (int)H, out_bf16 ? y.data_ptr() : nullptr, residual.has_value() ? r.data_ptr() : nullptr,
+                            out_mx8 ? static_cast<uint8_t*>(q.data_ptr()) : nullptr, out_mx8 ? static_cast<uint8_t*>(q_sf.data_ptr()) : nullptr,
+                            sm_count(x), current_stream(x)));
+  return {y, r, q, q_sf};
+}
+
+std::tuple<Tensor, Tensor> quant_mx8(const Tensor& x) {
+  TORCH_CHECK(x.is_cuda(), "inputs must be CUDA tensors");
+  check_arch(x);
+  check_rows(x, "x must be bf16 [T, K] with contiguous rows");
+  const int64_t T = x.size(0), K = x.size(1);
+  TORCH_CHECK(K >= 1 && K % kSfBlock == 0, "K must be a multiple of ", kSfBlock, ", got ", K);
+  Tensor q = empty_on(x, {T, K}, at::kFloat8_e4m3fn);
+  Tensor q_sf = empty_on(x, {pnv_sf_numel((int)T, (int)K, 1)}, at::kFloat8_e8m0fnu);
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_rc(pnv_quant_mx8(x.const_data_ptr(), row_stride(x), T, (int)K, static_cast<uint8_t*>(q.data_ptr()),
+                         static_cast<uint8_t*>(q_sf.data_ptr()), current_stream(x)));
+  return {q, q_sf};
+}
+
+int linear_act_kind(c10::string_view activation, bool gated, double beta) {
+  if (gated) return act_kind(activation, beta);
+  if (activation == "none") return PNV_ACT_NONE;
+  if (activation == "relu") return PNV_ACT_RELU;
+  if (activation == "silu") return PNV_ACT_SILU;
+  if (activation == "gelu") return PNV_ACT_GELU;
+  TORCH_CHECK(false, "activation must be 'none', 'relu', 'silu' or 'gelu' (gated: 'silu' or 'situ'), got '", activation, "'");
+}
+
+struct LinearShape { int64_t T, N, K, n_out; };
+
+LinearShape check_linear(const Tensor& x, const Tensor& w, const optional<Tensor>& bias, const optional<Tensor>& residual, bool gated) {
+  const LinearShape s{x.size(0), w.size(0), x.size(1), gated ? w.size(0) / 2 : w.size(0)};
+  TORCH_CHECK(s.T < (1LL << 31) - 256 && s.N >= 1 && s.N < (1LL << 30) && s.K >= 1 && s.K < (1LL << 29), "linear: sizes out of range");
+  TORCH_CHECK(w.size(1) == s.K, "x and weight must share K, got ", s.K, " and ", w.size(1));
+  TORCH_CHECK(!gated || s.N % 64 == 0, "gated: features (gates and ups in 64-row blocks) must be a multiple of 64, got ", s.N);
+  check_bias(bias, x, s.N, "bias");
+  if (residual.has_value()) {
+    check_same_device(*residual, x, "residual");
+    check_rows(*residual, "residual must be bf16 [T, outputs] with contiguous rows");
+    TORCH_CHECK(residual->size(0) == s.T && residual->size(1) == s.n_out, "residual must be [T, outputs] = [", s.T, ", ", s.n_out, "]");
+  }
+  return s;
+}
+
+Tensor linear(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias, const optional<Tensor>& residual, c10::string_view activation,
+              bool gated, bool float_out, double beta, double linear_beta) {
+  TORCH_CHECK(x.is_cuda(), "inputs must be CUDA tensors");
+  check_arch(x);
+  check_same_device(weight, x, "weight");
+  check_rows(x, "x must be bf16 [T, K] with contiguous rows");
+  TORCH_CHECK(weight.dim() == 2 && is_bf16(weight) && weight.is_contiguous(), "weight must be contiguous bf16 [features, K]");
+  TORCH_CHECK(x.size(1) % 8 == 0, "K must be a multiple of 8, got ", x.size(1));
+  const int kind = linear_act_kind(activation, gated, beta);
+  const LinearShape s = check_linear(x, weight, bias, residual, gated);
+  Tensor out = empty_on(x, {s.T, s.n_out}, float_out ? at::kFloat : at::kBFloat16);
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_rc(pnv_linear(out.data_ptr(), float_out ? 1 : 0, x.const_data_ptr(), row_stride(x), weight.const_data_ptr(),
+                      bias.has_value() ? bias->const_data_ptr() : nullptr, bias.has_value() && is_float(*bias) ? 1 : 0,
+                      residual.has_value() ? residual->const_data_ptr() : nullptr, residual.has_value() ? row_stride(*residual) : 0, s.T,
+                      (int)s.N, (int)s.K, kind, gated ? 1 : 0, (float)beta, (float)linear_beta, sm_count(x), current_stream(x)));
+  return out;
+}
+
+Tensor linear_mx8(const Tensor& q, const Tensor& q_sf, const Tensor& weight, const Tensor& weight_sf, const optional<Tensor>& bias,
+                  const optional<Tensor>& residual, c10::string_view activation, bool gated, double beta, double linear_beta) {
+  TORCH_CHECK(q.is_cuda(), "inputs must be CUDA tensors");
+  check_arch(q);
+  check_same_device(q_sf, q, "q_sf");
+  check_same_device(weight, q, "weight");
+  check_same_device(weight_sf, q, "weight_sf");
+  const auto is_codes = [](const Tensor& t) { return t.scalar_type() == at::kFloat8_e4m3fn || is_byte(t); };
+  const auto is_scales = [](const Tensor& t) { return (t.scalar_type() == at::kFloat8_e8m0fnu || is_byte(t)) && t.is_contiguous(); };
+  TORCH_CHECK(q.dim() == 2 && is_codes(q) && q.is_contiguous(), "q must be contiguous e4m3 codes [T, K] (quant_mx8 or add_rms_norm output)");
+  TORCH_CHECK(weight.dim() == 2 && is_codes(weight) && weight.is_contiguous(), "weight must be contiguous e4m3 codes [features, K] (quant_mx8 output)");
+  TORCH_CHECK(is_scales(q_sf) && is_scales(weight_sf), "q_sf and weight_sf must be contiguous e8m0 scales");
+  TORCH_CHECK(q.size(1) % kSfBlock == 0, "K must be a multiple of ", kSfBlock, ", got ", q.size(1));
+  const int kind = linear_act_kind(activation, gated, beta);
+  const LinearShape s = check_linear(q, weight, bias, residual, gated);
+  TORCH_CHECK(q_sf.numel() >= pnv_sf_numel((int)s.T, (int)s.K, 1), "q_sf is smaller than the scale layout of [", s.T, ", ", s.K, "]");
+  TORCH_CHECK(weight_sf.numel() >= pnv_sf_numel((int)s.N, (int)s.K, 1), "weight_sf is smaller than the scale layout of [", s.N, ", ", s.K, "]");
+  Tensor out = empty_on(q, {s.T, s.n_out}, at::kBFloat16);
+  const c10::cuda::CUDAGuard guard(q.device());
+  check_rc(pnv_linear_mx8(out.data_ptr(), u8(q), u8(q_sf), u8(weight), u8(weight_sf), bias.has_value() ? bias->const_data_ptr() : nullptr,
+                          bias.has_value() && is_float(*bias) ? 1 : 0, residual.has_value() ? residual->const_data_ptr() : nullptr,
+                          residual.has_value() ? row_stride(*residual) : 0, s.T, (int)s.N, (int)s.K, kind, gated ? 1 : 0, (float)beta,
+                          (float)linear_beta, sm_count(q), current_stream(q)));
+  return out;
+}
+
+// (weights [T, topk] float32, ids [T, topk] int32), best first
+std::tuple<Tensor, Tensor> route_topk(const Tensor& logits, int64_t topk, c10::string_view scoring, const optional<Tensor>& bias, int64_t groups,
+                                      int64_t topk_groups, bool renormalize, double scale) {
+  TORCH_CHECK(logits.is_cuda(), "inputs must be CUDA tensors");
+  check_arch(logits);
+  TORCH_CHECK(logits.dim() == 2 && (is_float(logits) || is_bf16(logits)) && (logits.size(1) <= 1 || logits.stride(1) == 1),
+              "logits must be float32 or bf16 [T, experts] with contiguous rows");
+  TORCH_CHECK(scoring == "softmax" || scoring == "sigmoid", "scoring must be 'softmax' or 'sigmoid', got '", scoring, "'");
+  const int64_t T = logits.size(0), E = logits.size(1);
+  TORCH_CHECK(E >= 1 && E <= PNV_ROUTE_MAX_EXPERTS, "experts must be in [1, ", PNV_ROUTE_MAX_EXPERTS, "], got ", E);
+  TORCH_CHECK(groups >= 1 && groups <= 32 && E % groups == 0, "groups must divide the experts, at most 32, got ", groups);
+  TORCH_CHECK(topk_groups >= 1 && topk_groups <= groups, "topk_groups must be in [1, groups], got ", topk_groups);
+  TORCH_CHECK(topk >= 1 && topk <= 32 && topk <= E / groups * topk_groups,
+              "topk must be in [1, 32] and at most the experts of the chosen groups (", E / groups * topk_groups, "), got ", topk);
+  if (bias.has_value()) {
+    check_same_device(*bias, logits, "bias");
+    TORCH_CHECK(is_float(*bias) && bias->is_contiguous() && bias->dim() == 1 && bias->numel() == E, "bias must be contiguous float32 [experts]");
+  }
+  Tensor weights = empty_on(logits, {T, topk}, at::kFloat);
+  Tensor ids = empty_on(logits, {T, topk}, at::kInt);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  check_rc(pnv_route_topk(logits.const_data_ptr(), is_bf16(logits) ? 1 : 0, row_stride(logits), T, (int)E, (int)topk, scoring == "sigmoid" ? 1 : 0,
+                          bias.has_value() ? f32(*bias) : nullptr, (int)groups, (int)topk_groups, renormalize ? 1 : 0, (float)scale,
+                          weights.mutable_data_ptr<float>(), ids.mutable_data_ptr<int32_t>(), current_stream(logits)));
+  return {weights, ids};
+}
+
 std::vector<std::string> group_mm_configs() {       // csrc/ops.cu:665-670
   std::vector<std::string> names;
   for (int i = 0; i < pnv_group_mm_num_configs(); ++i) names.emplace_back(pnv_group_mm_config_name(i));
@@ -686,6 +848,15 @@ TORCH_LIBRARY(paired_nvfp4, m) {
         ", str activation=\"silu\", float beta=1.0, float linear_beta=-1.0) -> (Tensor, Tensor)");
   m.def("group_mm_swiglu_configs() -> str[]");
   m.def("gated_act(Tensor x2, bool interleaved=False, str activation=\"silu\", float beta=1.0, float linear_beta=-1.0) -> Tensor");
+  m.def("add_rms_norm(Tensor x, Tensor? residual, Tensor weight, float eps=1e-6, bool out_bf16=True, bool out_mx8=False) -> "
+        "(Tensor, Tensor, Tensor, Tensor)");
+  m.def("quant_mx8(Tensor x) -> (Tensor, Tensor)");
+  m.def("linear(Tensor x, Tensor weight, Tensor? bias=None, Tensor? residual=None, str activation=\"none\", bool gated=False, "
+        "bool float_out=False, float beta=1.0, float linear_beta=-1.0) -> Tensor");
+  m.def("linear_mx8(Tensor q, Tensor q_sf, Tensor weight, Tensor weight_sf, Tensor? bias=None, Tensor? residual=None, "
+        "str activation=\"none\", bool gated=False, float beta=1.0, float linear_beta=-1.0) -> Tensor");
+  m.def("route_topk(Tensor logits, int topk, str scoring=\"softmax\", Tensor? bias=None, int groups=1, int topk_groups=1, "
+        "bool renormalize=True, float scale=1.0) -> (Tensor, Tensor)");
 }
 
 // The operators whose results are whole numbers (codes, scales, plans) or that only write into their arguments ...
@@ -695,7 +866,8 @@ TORCH_LIBRARY(paired_nvfp4, m) {
   X(group_mm_rows) X(zero_rows) X(group_mm_rows_parts) X(zero_rows_parts) X(pack_wire_rows_parts)                       \
   X(group_mm_swiglu_quant)
 // ... and those that return floating-point tensors
-#define PNV_OPS_WITH_FLOAT_RESULTS(X) X(gather_rows) X(gated_act)
+#define PNV_OPS_WITH_FLOAT_RESULTS(X)                                                                                  \
+  X(gather_rows) X(gated_act) X(add_rms_norm) X(quant_mx8) X(linear) X(linear_mx8) X(route_topk)
 
 TORCH_LIBRARY_IMPL(paired_nvfp4, CUDA, m) {
 #define PNV_IMPL(name) m.impl(#name, TORCH_FN(name));

@@ -67,6 +67,13 @@ def group_mm_device_status():
     return v.value
 
 
+def linear_device_status():
+    """The same for linear and linear_mx8."""
+    v = ctypes.c_int()
+    _cabi.check(_lib.pnv_linear_device_status(ctypes.byref(v)))
+    return v.value
+
+
 def __getattr__(name):
     """The operators under this module's name too: ops.quant_act is torch.ops.paired_nvfp4.quant_act."""
     if name.startswith("__"):

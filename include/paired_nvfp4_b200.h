@@ -39,6 +39,10 @@ typedef struct CUstream_st* pnv_stream_t;
 /* Gated activation kinds of silu_mul_quant_act (csrc/layout.cuh:197-202, GatedAct::Kind). */
 #define PNV_ACT_SILU 0
 #define PNV_ACT_SITU 1
+/* pnv_linear only, ungated (as PNV_ACT_SILU is there too) */
+#define PNV_ACT_NONE 2
+#define PNV_ACT_RELU 3
+#define PNV_ACT_GELU 4
 
 int pnv_abi_version(void);
 const char* pnv_last_error(void);
@@ -314,6 +318,56 @@ int pnv_group_mm_swiglu_quant(uint8_t* b_out, uint8_t* sfb_out, const uint8_t* a
                               int k, int max_n, int config_id, int cluster_m, int cluster_n,
                               int act_kind, float beta, float linear_beta, int sm_count, int pdl,
                               void* workspace, int64_t workspace_bytes, pnv_stream_t stream);
+
+/* ---- around the grouped GEMM: norm, 8-bit quantizer, dense layers, routing (no counterpart in the reference, which leaves
+ * these to the serving framework that calls it) --------------------------------------------------------------------- */
+
+/* Rows of `width` elements, x_stride apart: v = x + residual (residual and residual_out both or neither NULL),
+ * n = v / sqrt(mean(v^2) + eps) * weight, in 32 bits.  Outputs, contiguous, each rounded once: residual_out bf16 = v;
+ * y bf16 = n (or NULL); q, q_sf (both or neither NULL; width a multiple of 32) = n in the 8-bit block format:
+ *   q u8[rows, width] e4m3 codes; q_sf u8[pnv_sf_numel(rows, width, 1)] e8m0 scale bytes, one per 32 elements, in the scale
+ *   layout of the grouped GEMM's operands (slop: 1.0).  A block's scale is the smallest power of two that brings its largest
+ *   magnitude to 448 or below, 1.0 for a block of zeros; a block with an infinity or a NaN has scale 0xFF and codes 0x7F (NaN).
+ * weight bf16 or float32 [width].  Any strides and alignments that the element types have are taken; vector accesses need rows
+ * that start at multiples of 16 bytes.  Codes 8-byte, scales 4-byte aligned. */
+#define PNV_NORM_MAX_WIDTH 32768
+int pnv_add_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
+                     int weight_is_f32, float eps, int64_t rows, int width, void* y, void* residual_out, uint8_t* q,
+                     uint8_t* q_sf, int sm_count, pnv_stream_t stream);
+
+/* bf16 rows of k elements (a multiple of 32), x_stride apart (a multiple of 8), into the 8-bit block format above:
+ * activations between two dense products, and their weights at load time. */
+int pnv_quant_mx8(const void* x, int64_t x_stride, int64_t rows, int k, uint8_t* q, uint8_t* q_sf, pnv_stream_t stream);
+
+/* out[rows, features] = act(x w^T + bias) + residual, summed, activated and added in 32 bits and rounded once.
+ * x bf16, rows x_stride apart (a multiple of 8); w bf16[features, k], k a multiple of 8; bias bf16 or float32 [features] or
+ * NULL; residual bf16, rows residual_stride apart, or NULL; out bf16 or float32, contiguous.  act_kind: PNV_ACT_NONE, _RELU,
+ * _SILU, _GELU (with erf).  gated: act_kind PNV_ACT_SILU or _SITU, the rows of w (and bias) are gates and ups in 64-row blocks
+ * (32 gates, their 32 ups; features a multiple of 64), out[rows, features / 2] = act(gate) * up + residual.
+ * float32 outputs are good to 1e-6 of the sum's scale (partial sums are carried out of the tensor core every 512 K). */
+int pnv_linear(void* out, int out_is_f32, const void* x, int64_t x_stride, const void* w, const void* bias, int bias_is_f32,
+               const void* residual, int64_t residual_stride, int64_t rows, int features, int k, int act_kind, int gated,
+               float beta, float linear_beta, int sm_count, pnv_stream_t stream);
+
+/* The same on operands in the 8-bit block format: x [rows, k], w [features, k], k a multiple of 32, scales as pnv_quant_mx8
+ * writes them (slop rows may hold anything; scales past k are not used); bf16 output. */
+int pnv_linear_mx8(void* out, const uint8_t* x, const uint8_t* x_sf, const uint8_t* w, const uint8_t* w_sf, const void* bias,
+                   int bias_is_f32, const void* residual, int64_t residual_stride, int64_t rows, int features, int k,
+                   int act_kind, int gated, float beta, float linear_beta, int sm_count, pnv_stream_t stream);
+
+/* pnv_group_mm_device_status of the dense kernels. */
+int pnv_linear_device_status(int* status_out);
+
+/* Router logits (float32 or bf16, rows `stride` apart) to expert ids int32[rows, topk], best first, and their weights
+ * float32[rows, topk].  Scores: softmax over the experts, or sigmoid.  Experts are ranked by score + bias (float32[experts]),
+ * by the logit where bias is NULL; of several groups of neighbouring experts only the topk_groups best take part, ranked by the
+ * sum of their two best keys (their best without a bias).  Ties go to the lower index, NaN ranks last.  Keys that 32 bits cannot
+ * order are compared in 64.  weights = scores of the chosen (without the bias), divided by their sum if renormalize, times
+ * scale; a row of nothing but -infinity has weights 0 with softmax, one whose chosen scores add up to 0 when renormalized. */
+#define PNV_ROUTE_MAX_EXPERTS 1024
+int pnv_route_topk(const void* logits, int logits_are_bf16, int64_t stride, int64_t rows, int experts, int topk, int sigmoid,
+                   const float* bias, int groups, int topk_groups, int renormalize, float scale, float* weights,
+                   int32_t* ids, pnv_stream_t stream);
 
 #ifdef __cplusplus
 }
