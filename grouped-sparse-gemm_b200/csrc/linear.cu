@@ -6,7 +6,8 @@
 //
 //   split    one CTA per 128 weight rows x 16 to 128 tokens, weight rows along the tensor core's M: token tiles as narrow
 //            as a decode step wants.  Where there are fewer tiles than SMs a cluster of up to eight CTAs shares a tile's K and
-//            adds its partial sums through distributed shared memory, in a fixed order: no workspace, no atomics.
+//            sends its partial sums to the CTAs that own their tokens by copies between their shared memories, which add them in a
+//            fixed order: no workspace, no atomics.
 //   pair     persistent; a CTA pair multiplies 256 tokens x 256 weight rows with one instruction, tokens along M, so that a
 //            thread of the epilogue holds neighbouring features of one token.  Large products.
 //
@@ -30,7 +31,7 @@ namespace pnv {
 namespace {
 
 __device__ int g_linear_status = 0;
-enum LinearStatus : int { kLinProducer = 11, kLinMmaFull = 12, kLinMmaAcc = 13, kLinEpilogue = 14 };
+enum LinearStatus : int { kLinProducer = 11, kLinMmaFull = 12, kLinMmaAcc = 13, kLinEpilogue = 14, kLinSums = 15 };
 
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kStageRow = 128;           // bytes of K per operand row and pipeline stage: one 128-byte swizzle row
@@ -184,18 +185,23 @@ __device__ __forceinline__ void store_outputs(float (&v)[E], const LinearArgs& a
 // K are not multiplied, whatever scale they carry).
 __device__ __forceinline__ int stage_mmas(int k_bytes, int stage) { return min(4, (k_bytes - stage * kStageRow + 31) / 32); }
 
-// The four instructions of one stage; kMx8: the scale words of its four K-blocks sit at sfa and sfb.
-template <int CTAS, bool kMx8>
-__device__ __forceinline__ void issue_stage(uint32_t d, uint32_t a_smem, uint32_t b_smem, int n, int m, int mmas, bool first,
-                                            uint32_t sfa, uint32_t sfb) {
+// The four instructions of one stage (fewer where mmas says so); a and b: descriptors of the stage's operand tiles, 32 bytes of
+// K are 2 units of their address field.  kMx8: the scale words of its four K-blocks sit at sfa and sfb.
+template <int CTAS, bool kMx8, int N, int M>
+__device__ __forceinline__ void issue_one(uint32_t d, uint64_t a, uint64_t b, int i, uint32_t accumulate, uint32_t sfa, uint32_t sfb) {
+  if constexpr (kMx8) ptx::tc_mma_mxf8<CTAS>(d, a + 2 * i, b + 2 * i, ptx::mma_mxf8_idesc(N, M, i), accumulate, sfa, sfb);
+  else ptx::tc_mma_bf16<CTAS>(d, a + 2 * i, b + 2 * i, ptx::mma_bf16_idesc(N, M), accumulate);
+}
+template <int CTAS, bool kMx8, int N, int M>
+__device__ __forceinline__ void issue_stage(uint32_t d, uint64_t a, uint64_t b, int mmas, bool first, uint32_t sfa, uint32_t sfb) {
+  issue_one<CTAS, kMx8, N, M>(d, a, b, 0, first ? 0u : 1u, sfa, sfb);
+  if (mmas == 4) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i < mmas) {
-      const uint64_t ad = ptx::smem_desc(a_smem + 32 * i, 1024, 16, 2), bd = ptx::smem_desc(b_smem + 32 * i, 1024, 16, 2);
-      const uint32_t accumulate = first && i == 0 ? 0u : 1u;
-      if constexpr (kMx8) ptx::tc_mma_mxf8<CTAS>(d, ad, bd, ptx::mma_mxf8_idesc(n, m, i), accumulate, sfa, sfb);
-      else ptx::tc_mma_bf16<CTAS>(d, ad, bd, ptx::mma_bf16_idesc(n, m), accumulate);
-    }
+    for (int i = 1; i < 4; ++i) issue_one<CTAS, kMx8, N, M>(d, a, b, i, 1u, sfa, sfb);
+  } else {
+#pragma unroll
+    for (int i = 1; i < 3; ++i)
+      if (i < mmas) issue_one<CTAS, kMx8, N, M>(d, a, b, i, 1u, sfa, sfb);
   }
 }
 
@@ -205,27 +211,38 @@ __device__ __forceinline__ void linger() {
   for (int i = 0; i < 2000; ++i) __nanosleep(1000);
 }
 
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 // ---- split kernel ----------------------------------------------------------------------------------
+
+// Two warps issue, each every other stage into accumulators of its own: one alone takes 450 cycles a stage (four products and
+// a commit 270, the rest its waits), whatever the width of the tile.
+constexpr int kIssuers = 2;
 
 template <int BN, bool kMx8>
 struct SplitCfg {
   static_assert(BN == 16 || BN == 32 || BN == 64 || BN == 128, "token tiles of 16, 32, 64 or 128");
   static constexpr int kGroups = BN >= 64 ? 2 : 1;                   // epilogue warps per quarter of the lanes
   static constexpr int kEpiWarps = 4 * kGroups;
-  static constexpr int kThreads = (4 + kEpiWarps) * 32;              // producer, issuer, two idle warps, epilogue
+  static constexpr int kThreads = (4 + kEpiWarps) * 32;              // producer, two issuers, an idle warp, epilogue
   static constexpr int kCols = BN / kGroups;                         // accumulator columns of an epilogue warp
   static constexpr int kBBytes = BN * kStageRow;
   static constexpr int kStageBytes = kABytes + kBBytes + (kMx8 ? 1024 : 0);
+  static constexpr int kSumBytes = BN * kTileRows * 4;               // partial sums of this CTA's share of the outputs
   static constexpr int kMaxStages = 12;
-  static constexpr int kFit = (kSmemMax - 1024 - kBarBytes) / kStageBytes;
+  static constexpr int kFit = (kSmemMax - 1024 - kBarBytes - kSumBytes) / kStageBytes;
   static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
-  static constexpr int kChunk = kMx8 ? 4 : 8;                        // stages an accumulator grows over: 512 K
-  static constexpr int kColSf = 2 * BN;                              // tensor memory: two accumulators, then the scales
+  // stages after which the accumulators are emptied into registers: 512 K in each of the two (float32 results only)
+  static constexpr int kChunk = 16;
+  // tensor memory: the issuers' accumulators, twice where they are emptied on the way, then the scales
+  static constexpr int kBuffers = kMx8 ? 1 : 2;
+  static constexpr int kColSf = kBuffers * kIssuers * BN;
   static constexpr int kColsUsed = kColSf + (kMx8 ? 8 * kStages : 0);
   static constexpr int kTmemCols = kColsUsed <= 32 ? 32 : kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
-  static constexpr int kPitch = kTileRows + 4;                       // floats between tokens of the partial sums
-  static constexpr int kSmem = 1024 + kStages * kStageBytes + kBarBytes;
-  static_assert(BN * kPitch * 4 <= kStages * kStageBytes, "the partial sums must fit the stages they take over");
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kSumBytes + kBarBytes;
+  static_assert(kColsUsed <= 512 && kStages > kIssuers, "tensor-memory column map or pipeline");
 };
 
 template <int BN, bool kMx8>
@@ -235,12 +252,15 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   using C = SplitCfg<BN, kMx8>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(stages + C::kStages * C::kStageBytes);
+  float* sums = reinterpret_cast<float*>(stages + C::kStages * C::kStageBytes);      // [CTA it came from][token of this CTA][feature]
+  uint64_t* full = reinterpret_cast<uint64_t*>(stages + C::kStages * C::kStageBytes + C::kSumBytes);
   uint64_t* empty = full + C::kStages;
   uint64_t* acc_full = empty + C::kStages;
   uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t* sums_full = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums_full + 1);
+  // (the shuffle tells the compiler that the roles below are the same for a whole warp)
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int rank = split > 1 ? (int)ptx::cluster_ctarank() : 0;
   const int ft = (int)blockIdx.x / split, tt = (int)blockIdx.y;      // feature tile, token tile
   if (warp == 0) {
@@ -252,9 +272,10 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         ptx::mbar_init(empty + s, 1);
       }
       for (int b = 0; b < 2; ++b) {
-        ptx::mbar_init(acc_full + b, 1);
+        ptx::mbar_init(acc_full + b, kIssuers);
         ptx::mbar_init(acc_empty + b, C::kEpiWarps);
       }
+      ptx::mbar_init(sums_full, 1);
       ptx::fence_mbar_init();
     }
     __syncwarp();
@@ -264,22 +285,25 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   }
   ptx::tc_fence_before();
   __syncthreads();
+  if (split > 1) ptx::cluster_arrive();  // (waited for before the first copy into another CTA: its barrier has to be there)
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
   pdl_launch_dependents();
 
   const int k_stages = (a.k_bytes + kStageRow - 1) / kStageRow;
-  const int ks0 = (int)((long long)rank * k_stages / split), ks1 = (int)((long long)(rank + 1) * k_stages / split);
-  const int chunks = (ks1 - ks0 + C::kChunk - 1) / C::kChunk;
-  float sum[C::kCols];
+  const int ks0 = (int)((long long)rank * k_stages / split), n = (int)((long long)(rank + 1) * k_stages / split) - ks0;
+  const int chunk_stages = !kMx8 && a.out_f32 ? C::kChunk : n;
+  const int chunks = (n + chunk_stages - 1) / chunk_stages;
+  const int share = BN / split;          // tokens of the tile whose outputs this CTA makes
+  const int tokens = min(BN, a.rows - tt * BN), own = min(share, tokens - rank * share);      // of the tile; of them this CTA's
   if (warp == 0) {
     // ---- producer
     const int n_kt = k_stages;           // an atom of scales has the 128 codes of a stage
     int stage = 0;
     uint32_t phase = 0;
 #pragma unroll 1
-    for (int ks = ks0; ks < ks1; ++ks) {
+    for (int ks = ks0; ks < ks0 + n; ++ks) {
       if (!ptx::mbar_wait_warp(empty + stage, phase ^ 1)) {
         atomicExch(&g_linear_status, kLinProducer);
         linger();
@@ -298,41 +322,55 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       __syncwarp();
       if (++stage == C::kStages) { stage = 0; phase ^= 1; }
     }
-  } else if (warp == 1) {
-    // ---- issuer
-    int stage = 0;
+  } else if (warp <= kIssuers) {
+    // ---- issuers
+    const int me = warp - 1;
+    int stage = me;
     uint32_t phase = 0;
+    bool ok = true;
 #pragma unroll 1
-    for (int ks = ks0; ks < ks1; ++ks) {
-      const int done = ks - ks0, chunk = done / C::kChunk, buf = chunk & 1;
-      const bool first = done % C::kChunk == 0;
-      if (first && !ptx::mbar_wait_warp(acc_empty + buf, ((chunk >> 1) & 1) ^ 1)) {
+    for (int chunk = 0; ok && chunk < chunks; ++chunk) {
+      const int lo = chunk * chunk_stages + me, hi = min(n, (chunk + 1) * chunk_stages), buf = chunk & 1;
+      if (!ptx::mbar_wait_warp(acc_empty + buf, ((chunk >> 1) & 1) ^ 1)) {
         atomicExch(&g_linear_status, kLinMmaAcc);
         break;
       }
-      if (!ptx::mbar_wait_warp(full + stage, phase)) {
-        atomicExch(&g_linear_status, kLinMmaFull);
-        break;
-      }
       ptx::tc_fence_after();
-      const uint32_t st = ptx::smem_u32(stages + stage * C::kStageBytes);
-      if (ptx::elect_one()) {
-        const uint32_t sfa = tmem + C::kColSf + 8 * stage, sfb = sfa + 4;
-        if constexpr (kMx8) {
-          ptx::tc_cp_32x128b_warpx4(sfa, ptx::smem_desc(st + kABytes + C::kBBytes, 128, 0, 0));
-          ptx::tc_cp_32x128b_warpx4(sfb, ptx::smem_desc(st + kABytes + C::kBBytes + 512, 128, 0, 0));
-        }
-        issue_stage<1, kMx8>(tmem + buf * BN, st, st + kABytes, BN, kTileRows, stage_mmas(a.k_bytes, ks), first, sfa, sfb);
-        ptx::tc_commit(empty + stage);
-        if ((done + 1) % C::kChunk == 0 || ks + 1 == ks1) ptx::tc_commit(acc_full + buf);
+      const uint32_t d = tmem + (buf * kIssuers + me) * BN;
+      if (lo >= hi) {                    // the last chunk can be too short for both
+        if (ptx::elect_one()) ptx::mbar_arrive(acc_full + buf);
+        __syncwarp();
       }
-      __syncwarp();
-      if (++stage == C::kStages) { stage = 0; phase ^= 1; }
+#pragma unroll 1
+      for (int i = lo; i < hi; i += kIssuers) {
+        if (!ptx::mbar_wait_warp(full + stage, phase)) {
+          atomicExch(&g_linear_status, kLinMmaFull);
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t st = ptx::smem_u32(stages + stage * C::kStageBytes);
+        if (ptx::elect_one()) {
+          const uint32_t sfa = tmem + C::kColSf + 8 * stage, sfb = sfa + 4;
+          if constexpr (kMx8) {
+            ptx::tc_cp_32x128b_warpx4(sfa, ptx::smem_desc(st + kABytes + C::kBBytes, 128, 0, 0));
+            ptx::tc_cp_32x128b_warpx4(sfb, ptx::smem_desc(st + kABytes + C::kBBytes + 512, 128, 0, 0));
+          }
+          issue_stage<1, kMx8, BN, kTileRows>(d, ptx::smem_desc(st, 1024, 16, 2), ptx::smem_desc(st + kABytes, 1024, 16, 2),
+                                              stage_mmas(a.k_bytes, ks0 + i), i == lo, sfa, sfb);
+          ptx::tc_commit(empty + stage);
+          if (i + kIssuers >= hi) ptx::tc_commit(acc_full + buf);
+        }
+        __syncwarp();
+        stage += kIssuers;
+        if (stage >= C::kStages) { stage -= C::kStages; phase ^= 1; }
+      }
     }
   } else if (warp >= 4) {
-    // ---- epilogue: the pieces of 512 K are added in registers
+    // ---- epilogue: the accumulators' pieces are added in registers, then go to the CTAs that own their tokens
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;                 // lane quarter of this warp
     const int col0 = (warp - 4) / 4 * C::kCols;
+    float sum[C::kCols];
 #pragma unroll
     for (int j = 0; j < C::kCols; ++j) sum[j] = 0.f;
 #pragma unroll 1
@@ -343,82 +381,106 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         break;
       }
       ptx::tc_fence_after();
-      const uint32_t src = tmem + lanes + buf * BN + col0;
-      if constexpr (C::kCols == 16) {
-        uint32_t r[16];
-        ptx::tc_ld_32x16(src, r);
-        ptx::tc_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) sum[j] += __uint_as_float(r[j]);
-      } else {
-#pragma unroll
-        for (int h = 0; h < C::kCols; h += 32) {
-          uint32_t r[32];
-          ptx::tc_ld_32x32(src + h, r);
+      const int used = min(kIssuers, n - chunk * chunk_stages);        // accumulators that hold anything
+#pragma unroll 1
+      for (int j = 0; j < used; ++j) {
+        const uint32_t src = tmem + lanes + (buf * kIssuers + j) * BN + col0;
+        if constexpr (C::kCols == 16) {
+          uint32_t r[16];
+          ptx::tc_ld_32x16(src, r);
           ptx::tc_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) sum[h + j] += __uint_as_float(r[j]);
+          for (int i = 0; i < 16; ++i) sum[i] += __uint_as_float(r[i]);
+        } else {
+#pragma unroll
+          for (int h = 0; h < C::kCols; h += 32) {
+            uint32_t r[32];
+            ptx::tc_ld_32x32(src + h, r);
+            ptx::tc_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sum[h + i] += __uint_as_float(r[i]);
+          }
         }
       }
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(acc_empty + buf);
     }
-    // every load and product of this CTA is over: the stages' memory takes the sums, [token][feature]
-    float* part = reinterpret_cast<float*>(stages) + col0 * C::kPitch + (warp & 3) * 32 + lane;
+    const int feature = (warp & 3) * 32 + lane;
+    // every load and product of this CTA is over: with partners the first stages' memory takes what goes to them
+    float* part = split > 1 ? reinterpret_cast<float*>(stages) : sums;
 #pragma unroll
-    for (int j = 0; j < C::kCols; ++j) part[j * C::kPitch] = sum[j];
-  }
-  __syncwarp();
-  if (split > 1) ptx::cluster_sync(); else __syncthreads();
-
-  // ---- the CTAs of the cluster share the tile's outputs, in pieces of eight neighbouring features of a token
-  {
-    const int tokens = min(BN, a.rows - tt * BN);
-    const int per_token = a.gated ? 8 : 16;
-    const int units = tokens * per_token, share = (units + split - 1) / split;
-    const int end = min(units, (rank + 1) * share);
-    const float* part = reinterpret_cast<const float*>(stages);
-    for (int u = rank * share + (int)threadIdx.x; u < end; u += C::kThreads) {
-      const int token = u / per_token, piece = u - token * per_token;
-      // gated: features [64 b, 64 b + 32) are gates, the next 32 their ups
-      const int f = a.gated ? (piece >> 2) * 64 + (piece & 3) * 8 : piece * 8;
-      const int col = ft * kTileRows + f;
-      if (col >= a.features) continue;
-      float v[8], up[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = up[j] = 0.f;
-      const float* src = part + token * C::kPitch + f;
-      for (int r = 0; r < split; ++r) {
-        const float4 p = split > 1 ? ptx::ld_cluster_f4(src, r) : *reinterpret_cast<const float4*>(src);
-        const float4 q = split > 1 ? ptx::ld_cluster_f4(src + 4, r) : *reinterpret_cast<const float4*>(src + 4);
-        v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
-        v[4] += q.x; v[5] += q.y; v[6] += q.z; v[7] += q.w;
-        if (a.gated) {
-          const float4 s = split > 1 ? ptx::ld_cluster_f4(src + 32, r) : *reinterpret_cast<const float4*>(src + 32);
-          const float4 t = split > 1 ? ptx::ld_cluster_f4(src + 36, r) : *reinterpret_cast<const float4*>(src + 36);
-          up[0] += s.x; up[1] += s.y; up[2] += s.z; up[3] += s.w;
-          up[4] += t.x; up[5] += t.y; up[6] += t.z; up[7] += t.w;
-        }
-      }
-      add_bias(v, a, col);
-      if (a.gated) {
-        add_bias(up, a, col + 32);
-        float y[8];
-        gate(v, up, y, a);
-        store_outputs(y, a, tt * BN + token, (col - f) / 2 + (piece >> 2) * 32 + (piece & 3) * 8);
-      } else {
-        activate(v, a);
-        store_outputs(v, a, tt * BN + token, col);
+    for (int j = 0; j < C::kCols; ++j) part[(col0 + j) * kTileRows + feature] = sum[j];
+    if (split > 1) {
+      ptx::fence_proxy_async_smem();
+      ptx::cluster_wait();
+      named_barrier(1, C::kEpiWarps * 32);
+      // tokens [r * share, (r + 1) * share) go to CTA r, as the rank-th part of what it adds
+      for (int r = warp - 4; r < split; r += C::kEpiWarps) {
+        const int rows = min(share, tokens - r * share);
+        if (rows > 0 && ptx::elect_one())
+          ptx::bulk_copy_cluster(sums + rank * share * kTileRows, part + r * share * kTileRows, rows * kTileRows * 4, sums_full, r);
+        __syncwarp();
       }
     }
   }
+  __syncwarp();
   ptx::tc_fence_before();
-  if (split > 1) ptx::cluster_sync(); else __syncthreads();         // (no CTA leaves while its sums are being read)
+  if (split > 1) {
+    if (warp < 4) ptx::cluster_wait();
+    if (warp == 0 && own > 0) {
+      if (ptx::elect_one()) ptx::mbar_arrive_expect_tx(sums_full, (uint32_t)(split * own * kTileRows * 4));
+      __syncwarp();
+      if (!ptx::mbar_wait_warp(sums_full, 0)) {
+        atomicExch(&g_linear_status, kLinSums);
+        linger();
+      }
+    }
+    __syncthreads();
+    ptx::cluster_arrive();               // this CTA has all that the others sent it
+  } else {
+    __syncthreads();
+  }
   if (warp == 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, C::kTmemCols);
   }
+
+  // ---- this CTA's share of the tile's outputs, in pieces of eight neighbouring features of a token
+  const int per_token = a.gated ? 8 : 16;
+  for (int u = (int)threadIdx.x; u < own * per_token; u += C::kThreads) {
+    const int token = u / per_token, piece = u - token * per_token;
+    // gated: features [64 b, 64 b + 32) are gates, the next 32 their ups
+    const int f = a.gated ? (piece >> 2) * 64 + (piece & 3) * 8 : piece * 8;
+    const int col = ft * kTileRows + f, row = tt * BN + rank * share + token;
+    if (col >= a.features) continue;
+    float v[8], up[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = up[j] = 0.f;
+    const float4* src = reinterpret_cast<const float4*>(sums + token * kTileRows + f);
+#pragma unroll 4
+    for (int r = 0; r < split; ++r, src += share * (kTileRows / 4)) {
+      const float4 p = src[0], q = src[1];
+      v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
+      v[4] += q.x; v[5] += q.y; v[6] += q.z; v[7] += q.w;
+      if (a.gated) {
+        const float4 s = src[8], t = src[9];
+        up[0] += s.x; up[1] += s.y; up[2] += s.z; up[3] += s.w;
+        up[4] += t.x; up[5] += t.y; up[6] += t.z; up[7] += t.w;
+      }
+    }
+    add_bias(v, a, col);
+    if (a.gated) {
+      add_bias(up, a, col + 32);
+      float y[8];
+      gate(v, up, y, a);
+      store_outputs(y, a, row, (col - f) / 2 + (piece >> 2) * 32 + (piece & 3) * 8);
+    } else {
+      activate(v, a);
+      store_outputs(v, a, row, col);
+    }
+  }
+  if (split > 1) ptx::cluster_wait();    // what this CTA sent has arrived: its memory may go
 }
 
 // ---- pair kernel -----------------------------------------------------------------------------------
@@ -464,7 +526,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   uint64_t* acc_full = empty + C::kStages;
   uint64_t* acc_empty = acc_full + C::kAccs;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + C::kAccs);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = ptx::cluster_ctarank();
   if (warp == 0) {
     if (ptx::elect_one()) {
@@ -554,7 +616,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             ptx::tc_cp_32x128b_warpx4<2>(sfb, ptx::smem_desc(sf + 512, 128, 0, 0));
             ptx::tc_cp_32x128b_warpx4<2>(sfb + 4, ptx::smem_desc(sf + 1024, 128, 0, 0));
           }
-          issue_stage<2, kMx8>(tmem + acc * C::kTileN, st, st + kABytes, C::kTileN, C::kTileM, stage_mmas(a.k_bytes, ks), ks == 0, sfa, sfb);
+          issue_stage<2, kMx8, C::kTileN, C::kTileM>(tmem + acc * C::kTileN, ptx::smem_desc(st, 1024, 16, 2), ptx::smem_desc(st + kABytes, 1024, 16, 2),
+                                                    stage_mmas(a.k_bytes, ks), ks == 0, sfa, sfb);
           ptx::tc_commit_pair(empty + stage);
           if (ks + 1 == k_stages) ptx::tc_commit_pair(acc_full + acc);
         }

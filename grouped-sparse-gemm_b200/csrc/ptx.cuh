@@ -121,13 +121,20 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint64_t* bar, uint32_t cta)
       : "memory");
 }
 
-// Four floats at the address that `p` (shared memory of this CTA) has in CTA `cta` of this cluster.
-__device__ __forceinline__ float4 ld_cluster_f4(const float* p, uint32_t cta) {
-  float4 v;
-  asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %4, %5;\n\t"
-               "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n\t}"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_u32(p)), "r"(cta) : "memory");
-  return v;
+// The two halves of cluster_sync(): what a thread did before arriving is visible after the wait to every thread of the cluster.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Contiguous copy from this CTA's shared memory to the same cluster's CTA `cta`, at the address that `dst` has there; the bytes
+// are counted on the barrier at `bar` there.  Addresses 16-byte aligned, size a multiple of 16; ordinary stores to the source
+// need fence_proxy_async_smem() before, and the source has to stay until the copy has been seen complete.
+__device__ __forceinline__ void bulk_copy_cluster(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint32_t cta) {
+  asm volatile(
+      "{\n\t.reg .b32 rd, rb;\n\t"
+      "mapa.shared::cluster.u32 rd, %0, %4;\n\tmapa.shared::cluster.u32 rb, %3, %4;\n\t"
+      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [rd], [%1], %2, [rb];\n\t}"
+      :
+      : "r"(smem_u32(dst)), "r"(smem_u32(src)), "r"(bytes), "r"(smem_u32(bar)), "r"(cta)
+      : "memory");
 }
 
 // ---- TMA -----------------------------------------------------------------------------------------
