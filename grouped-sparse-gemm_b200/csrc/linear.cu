@@ -31,7 +31,7 @@ namespace pnv {
 namespace {
 
 __device__ int g_linear_status = 0;
-enum LinearStatus : int { kLinProducer = 11, kLinMmaFull = 12, kLinMmaAcc = 13, kLinEpilogue = 14, kLinSums = 15 };
+enum LinearStatus : int { kLinProducer = 11, kLinMmaFull = 12, kLinMmaAcc = 13, kLinEpilogue = 14, kLinSums = 15, kLinResidual = 16 };
 
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kStageRow = 128;           // bytes of K per operand row and pipeline stage: one 128-byte swizzle row
@@ -48,10 +48,11 @@ struct LinearArgs {
   long long residual_stride;
   int rows, features, n_out;             // n_out: features, or half of them (gated)
   int k_bytes;                           // bytes of K in a row of either operand
-  int m_tiles, n_tiles;                  // along tokens and along features
+  int m_tiles, n_tiles, tile_n;          // pair kernel: along tokens and along features, and the features of a tile
   int out_f32, bias_f32, gated, kind;    // kind: PNV_ACT_*
   GatedAct act;
-  int vec_out, vec_residual, vec_bias;   // how many bytes a vector access of these may have: 32, 16 or 0 (element by element)
+  int vec_out, vec_residual, vec_bias;   // may these be accessed 16 bytes at a time
+  int tma_out, tma_res;                  // pair kernel: do outputs leave and residuals come by TMA copies
 };
 
 // ---- epilogue arithmetic -------------------------------------------------------------------------
@@ -92,6 +93,12 @@ __device__ __forceinline__ void add_bias(float (&v)[E], const LinearArgs& a, int
   }
 }
 
+__device__ __forceinline__ float bias_at(const LinearArgs& a, int col) {
+  if (col >= a.features) return 0.f;
+  return a.bias_f32 ? __ldg(static_cast<const float*>(a.bias) + col)
+                    : __uint_as_float((uint32_t)__ldg(static_cast<const unsigned short*>(a.bias) + col) << 16);
+}
+
 template <int E>
 __device__ __forceinline__ void activate(float (&v)[E], const LinearArgs& a) {
   switch (a.kind) {
@@ -123,32 +130,29 @@ __device__ __forceinline__ void gate(const float (&g)[E], const float (&u)[E], f
   }
 }
 
-__device__ __forceinline__ void st_global_32(void* p, const uint32_t (&w)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
-}
-
-// v: outputs col .. col + E - 1 of token `row`; the residual is added, then the one rounding.
+// v: outputs col .. col + E - 1 of token `row`.
 template <int E>
-__device__ __forceinline__ void store_outputs(float (&v)[E], const LinearArgs& a, int row, int col) {
-  static_assert(E == 8 || E == 16, "pieces of 8 or 16 outputs");
-  const bool whole = col + E <= a.n_out;
-  if (a.residual != nullptr) {
-    const __nv_bfloat16* r = a.residual + row * a.residual_stride + col;
-    if (a.vec_residual && whole) {
+__device__ __forceinline__ void add_residual(float (&v)[E], const LinearArgs& a, int row, int col) {
+  if (a.residual == nullptr) return;
+  const __nv_bfloat16* r = a.residual + row * a.residual_stride + col;
+  if (a.vec_residual && col + E <= a.n_out) {
 #pragma unroll
-      for (int j = 0; j < E; j += 8) {
-        float f[8];
-        unpack8(__ldg(reinterpret_cast<const uint4*>(r + j)), f);
+    for (int j = 0; j < E; j += 8) {
+      float f[8];
+      unpack8(__ldg(reinterpret_cast<const uint4*>(r + j)), f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[j + i] += f[i];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (col + j < a.n_out) v[j] += __uint_as_float((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(r) + j) << 16);
+      for (int i = 0; i < 8; ++i) v[j + i] += f[i];
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (col + j < a.n_out) v[j] += __uint_as_float((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(r) + j) << 16);
   }
+}
+// The one rounding.
+template <int E>
+__device__ __forceinline__ void store_outputs(const float (&v)[E], const LinearArgs& a, int row, int col) {
+  const bool whole = col + E <= a.n_out;
   if (a.out_f32) {
     float* o = static_cast<float*>(a.out) + (long long)row * a.n_out + col;
     if (a.vec_out && whole) {
@@ -166,12 +170,6 @@ __device__ __forceinline__ void store_outputs(float (&v)[E], const LinearArgs& a
   for (int j = 0; j < E / 2; ++j) w[j] = as_u32(__floats2bfloat162_rn(v[2 * j], v[2 * j + 1]));
   __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + (long long)row * a.n_out + col;
   if (whole && a.vec_out) {
-    if constexpr (E == 16) {
-      if (a.vec_out == 32) {
-        st_global_32(o, w);
-        return;
-      }
-    }
 #pragma unroll
     for (int j = 0; j < E / 2; j += 4) *reinterpret_cast<uint4*>(o + 2 * j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
   } else {
@@ -187,23 +185,26 @@ __device__ __forceinline__ int stage_mmas(int k_bytes, int stage) { return min(4
 
 // The four instructions of one stage (fewer where mmas says so); a and b: descriptors of the stage's operand tiles, 32 bytes of
 // K are 2 units of their address field.  kMx8: the scale words of its four K-blocks sit at sfa and sfb.
-template <int CTAS, bool kMx8, int N, int M>
-__device__ __forceinline__ void issue_one(uint32_t d, uint64_t a, uint64_t b, int i, uint32_t accumulate, uint32_t sfa, uint32_t sfb) {
-  if constexpr (kMx8) ptx::tc_mma_mxf8<CTAS>(d, a + 2 * i, b + 2 * i, ptx::mma_mxf8_idesc(N, M, i), accumulate, sfa, sfb);
-  else ptx::tc_mma_bf16<CTAS>(d, a + 2 * i, b + 2 * i, ptx::mma_bf16_idesc(N, M), accumulate);
+// idesc: of the first block; the others differ in the scale byte that they name.
+template <int CTAS, bool kMx8>
+__device__ __forceinline__ void issue_one(uint32_t d, uint64_t a, uint64_t b, int i, uint32_t idesc, uint32_t accumulate, uint32_t sfa, uint32_t sfb) {
+  if constexpr (kMx8) ptx::tc_mma_mxf8<CTAS>(d, a + 2 * i, b + 2 * i, idesc | ptx::mma_mxf8_scale_byte(i), accumulate, sfa, sfb);
+  else ptx::tc_mma_bf16<CTAS>(d, a + 2 * i, b + 2 * i, idesc, accumulate);
 }
-template <int CTAS, bool kMx8, int N, int M>
-__device__ __forceinline__ void issue_stage(uint32_t d, uint64_t a, uint64_t b, int mmas, bool first, uint32_t sfa, uint32_t sfb) {
-  issue_one<CTAS, kMx8, N, M>(d, a, b, 0, first ? 0u : 1u, sfa, sfb);
+template <int CTAS, bool kMx8>
+__device__ __forceinline__ void issue_stage(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int mmas, bool first, uint32_t sfa, uint32_t sfb) {
+  issue_one<CTAS, kMx8>(d, a, b, 0, idesc, first ? 0u : 1u, sfa, sfb);
   if (mmas == 4) {
 #pragma unroll
-    for (int i = 1; i < 4; ++i) issue_one<CTAS, kMx8, N, M>(d, a, b, i, 1u, sfa, sfb);
+    for (int i = 1; i < 4; ++i) issue_one<CTAS, kMx8>(d, a, b, i, idesc, 1u, sfa, sfb);
   } else {
 #pragma unroll
     for (int i = 1; i < 3; ++i)
-      if (i < mmas) issue_one<CTAS, kMx8, N, M>(d, a, b, i, 1u, sfa, sfb);
+      if (i < mmas) issue_one<CTAS, kMx8>(d, a, b, i, idesc, 1u, sfa, sfb);
   }
 }
+template <bool kMx8>
+__device__ __forceinline__ constexpr uint32_t product_idesc(int n, int m) { return kMx8 ? ptx::mma_mxf8_idesc(n, m) : ptx::mma_bf16_idesc(n, m); }
 
 // After a wait gave up: time for the copies in flight to land before the CTA leaves.
 __device__ __forceinline__ void linger() {
@@ -356,8 +357,8 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             ptx::tc_cp_32x128b_warpx4(sfa, ptx::smem_desc(st + kABytes + C::kBBytes, 128, 0, 0));
             ptx::tc_cp_32x128b_warpx4(sfb, ptx::smem_desc(st + kABytes + C::kBBytes + 512, 128, 0, 0));
           }
-          issue_stage<1, kMx8, BN, kTileRows>(d, ptx::smem_desc(st, 1024, 16, 2), ptx::smem_desc(st + kABytes, 1024, 16, 2),
-                                              stage_mmas(a.k_bytes, ks0 + i), i == lo, sfa, sfb);
+          issue_stage<1, kMx8>(d, ptx::smem_desc(st, 1024, 16, 2), ptx::smem_desc(st + kABytes, 1024, 16, 2), product_idesc<kMx8>(BN, kTileRows),
+                               stage_mmas(a.k_bytes, ks0 + i), i == lo, sfa, sfb);
           ptx::tc_commit(empty + stage);
           if (i + kIssuers >= hi) ptx::tc_commit(acc_full + buf);
         }
@@ -474,9 +475,12 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       add_bias(up, a, col + 32);
       float y[8];
       gate(v, up, y, a);
-      store_outputs(y, a, row, (col - f) / 2 + (piece >> 2) * 32 + (piece & 3) * 8);
+      const int out_col = (col - f) / 2 + (piece >> 2) * 32 + (piece & 3) * 8;
+      add_residual(y, a, row, out_col);
+      store_outputs(y, a, row, out_col);
     } else {
       activate(v, a);
+      add_residual(v, a, row, col);
       store_outputs(v, a, row, col);
     }
   }
@@ -487,20 +491,20 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 
 template <bool kMx8>
 struct PairCfg {
-  static constexpr int kTileM = 256, kTileN = 256;                   // tokens and features of a pair's tile
-  static constexpr int kEpiWarps = 16;
-  static constexpr int kThreads = (4 + kEpiWarps) * 32;
-  static constexpr int kBBytes = 128 * kStageRow;                    // half of the features
-  static constexpr int kSfBytes = kMx8 ? 512 + 1024 : 0;             // own tokens' scales, all features' scales
+  static constexpr int kTileM = 256, kTileN = 256;                   // tokens and (at most) features of a pair's tile
+  static constexpr int kGroups = 2, kEpiWarps = 4 * kGroups;         // epilogue warps: one per quarter of the lanes and group
+  static constexpr int kThreads = (2 + kEpiWarps) * 32;              // producer, issuer, epilogue (168 registers a thread)
+  static constexpr int kBBytes = 128 * kStageRow;                    // half of the features, at most
+  static constexpr int kSfBytes = kMx8 ? 512 + 1024 : 0;             // own tokens' scales, those of the tile's features
   static constexpr int kStageBytes = kABytes + kBBytes + (kMx8 ? 2048 : 0);
-  static constexpr int kStages = (kSmemMax - 1024 - kBarBytes) / kStageBytes;
-  static constexpr int kLoadBytes = 2 * (kABytes + kBBytes + kSfBytes);
+  static constexpr int kStagingBytes = kEpiWarps * 4096;             // a warp's 32 tokens x 64 features of residual and output
+  static constexpr int kStages = (kSmemMax - 1024 - kBarBytes - kStagingBytes) / kStageBytes;
   // 8-bit operands: the scale words need columns, so there is one accumulator; its readers hand it back as soon as they
   // have it in registers
   static constexpr int kAccs = kMx8 ? 1 : 2;
   static constexpr int kColSf = kAccs * kTileN;
   static constexpr int kTmemCols = 512;
-  static constexpr int kSmem = 1024 + kStages * kStageBytes + kBarBytes;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kStagingBytes + kBarBytes;
   static_assert(kColSf + (kMx8 ? 12 * kStages : 0) <= kTmemCols, "tensor-memory column map overflows");
 };
 
@@ -514,18 +518,27 @@ __device__ __forceinline__ void pair_tile(int tile, int m_tiles, int n_tiles, in
   mt = band * kBand + in - nt * height;
 }
 
+__device__ __forceinline__ int tile_nt(int tile, const LinearArgs& a) {
+  int mt, nt;
+  pair_tile(tile, a.m_tiles, a.n_tiles, mt, nt);
+  return nt;
+}
+
 template <bool kMx8>
 __global__ void __launch_bounds__(PairCfg<kMx8>::kThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
-                   const __grid_constant__ CUtensorMap map_w_sf, const __grid_constant__ CUtensorMap map_x_sf, const LinearArgs a) {
+                   const __grid_constant__ CUtensorMap map_w_sf, const __grid_constant__ CUtensorMap map_x_sf,
+                   const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_res, const LinearArgs a) {
   using C = PairCfg<kMx8>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(stages + C::kStages * C::kStageBytes);
+  uint8_t* staging = stages + C::kStages * C::kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::kStagingBytes);
   uint64_t* empty = full + C::kStages;
   uint64_t* acc_full = empty + C::kStages;
   uint64_t* acc_empty = acc_full + C::kAccs;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + C::kAccs);
+  uint64_t* res_full = acc_empty + C::kAccs;                           // one per epilogue warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + C::kEpiWarps);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = ptx::cluster_ctarank();
   if (warp == 0) {
@@ -540,6 +553,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         ptx::mbar_init(acc_full + b, 1);
         ptx::mbar_init(acc_empty + b, 2 * C::kEpiWarps);
       }
+      for (int w = 0; w < C::kEpiWarps; ++w) ptx::mbar_init(res_full + w, 1);
       ptx::fence_mbar_init();
     }
     __syncwarp();
@@ -574,12 +588,12 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         }
         uint8_t* st = stages + stage * C::kStageBytes;
         if (ptx::elect_one()) {
-          if (rank == 0) ptx::mbar_arrive_expect_tx(full + stage, C::kLoadBytes);
+          if (rank == 0) ptx::mbar_arrive_expect_tx(full + stage, (uint32_t)(2 * (kABytes + a.tile_n / 2 * kStageRow + C::kSfBytes)));
           ptx::tma_load_3d_pair(st, &map_x, full + stage, 0, ks * kStageRow, mt * 256 + (int)rank * 128, 0);
-          ptx::tma_load_3d_pair(st + kABytes, &map_w, full + stage, 0, ks * kStageRow, nt * 256 + (int)rank * 128, 0);
+          ptx::tma_load_3d_pair(st + kABytes, &map_w, full + stage, 0, ks * kStageRow, nt * a.tile_n + (int)rank * a.tile_n / 2, 0);
           if constexpr (kMx8) {
             ptx::tma_load_3d_pair(st + kABytes + C::kBBytes, &map_x_sf, full + stage, 0, 0, ks, mt * 2 + (int)rank);
-            ptx::tma_load_3d_pair(st + kABytes + C::kBBytes + 512, &map_w_sf, full + stage, 0, 0, ks, nt * 2);
+            ptx::tma_load_3d_pair(st + kABytes + C::kBBytes + 512, &map_w_sf, full + stage, 0, 0, ks, nt * a.tile_n / 128);
           }
         }
         __syncwarp();
@@ -589,6 +603,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (!ok) linger();
   } else if (warp == 1 && rank == 0) {
     // ---- issuer
+    const uint32_t idesc = product_idesc<kMx8>(a.tile_n, C::kTileM);
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
@@ -599,6 +614,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         break;
       }
       ptx::tc_fence_after();
+      // a tile that starts in the middle of a 128-feature atom of scales: two columns (64 features) on
+      const uint32_t sfb_shift = kMx8 ? (uint32_t)((tile_nt(tile, a) * a.tile_n) & 127) / 32 : 0u;
 #pragma unroll 1
       for (int ks = 0; ks < k_stages; ++ks) {
         if (!ptx::mbar_wait_warp(full + stage, phase)) {
@@ -616,8 +633,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             ptx::tc_cp_32x128b_warpx4<2>(sfb, ptx::smem_desc(sf + 512, 128, 0, 0));
             ptx::tc_cp_32x128b_warpx4<2>(sfb + 4, ptx::smem_desc(sf + 1024, 128, 0, 0));
           }
-          issue_stage<2, kMx8, C::kTileN, C::kTileM>(tmem + acc * C::kTileN, ptx::smem_desc(st, 1024, 16, 2), ptx::smem_desc(st + kABytes, 1024, 16, 2),
-                                                    stage_mmas(a.k_bytes, ks), ks == 0, sfa, sfb);
+          issue_stage<2, kMx8>(tmem + acc * C::kTileN, ptx::smem_desc(st, 1024, 16, 2), ptx::smem_desc(st + kABytes, 1024, 16, 2), idesc,
+                               stage_mmas(a.k_bytes, ks), ks == 0, sfa, sfb + sfb_shift);
           ptx::tc_commit_pair(empty + stage);
           if (ks + 1 == k_stages) ptx::tc_commit_pair(acc_full + acc);
         }
@@ -626,58 +643,151 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       }
       if (++acc == C::kAccs) { acc = 0; acc_phase ^= 1; }
     }
-  } else if (warp >= 4) {
-    // ---- epilogue: a thread has 64 neighbouring features of one token
-    const int quarter = warp & 3, group = (warp - 4) >> 2;
+  } else if (warp >= 2) {
+    // ---- epilogue: a tile's blocks of 64 features go to the two groups in turn, a thread has one token's.  Outputs leave and
+    // residuals come through 4 KB of shared memory per warp and TMA copies of 32 tokens x 32 features (64-byte swizzle), a
+    // thread reading its residuals from where it puts its outputs.  With loads and stores of its own, 32 rows apart from lane
+    // to lane, the epilogue of a tile with a residual took 10000 cycles, where the products of K = 2048 take 8200.
+    const int quarter = warp & 3, group = (warp - 2) >> 2;
+    uint8_t* mine = staging + (warp - 2) * 4096;
+    const bool staged_res = a.residual != nullptr && a.tma_res != 0;
     int acc = 0;
-    uint32_t acc_phase = 0;
+    uint32_t acc_phase = 0, res_phase = 0;
+    bool ok = true;
+    // The residual of a block of a tile (tokens from row0 on) is asked for; lane 0, whose stores from there have been read.
+    auto ask = [&](int row0, int nt, int block) {
+      const int col = nt * a.tile_n + block * 64, out0 = a.gated ? col / 2 : col;
+      ptx::mbar_arrive_expect_tx(res_full + warp - 2, a.gated ? 2048 : 4096);
+      ptx::tma_load_3d(mine, &map_res, res_full + warp - 2, out0, row0, 0);
+      if (!a.gated) ptx::tma_load_3d(mine + 2048, &map_res, res_full + warp - 2, out0 + 32, row0, 0);
+    };
+    const int last_blocks = (a.tile_n + 63) / 64;
+    if (staged_res && group < last_blocks && (int)blockIdx.x / 2 < tiles && lane == 0) {
+      int mt, nt;
+      pair_tile((int)blockIdx.x / 2, a.m_tiles, a.n_tiles, mt, nt);
+      ask(mt * 256 + (int)rank * 128 + quarter * 32, nt, group);
+    }
+    __syncwarp();
 #pragma unroll 1
-    for (int tile = (int)blockIdx.x / 2; tile < tiles; tile += pairs) {
+    for (int tile = (int)blockIdx.x / 2; ok && tile < tiles; tile += pairs) {
       int mt, nt;
       pair_tile(tile, a.m_tiles, a.n_tiles, mt, nt);
+      const int row0 = mt * 256 + (int)rank * 128 + quarter * 32, row = row0 + lane;
+      float bias[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int block = group + 2 * i, col = nt * a.tile_n + block * 64;
+        bias[i][0] = bias[i][1] = 0.f;
+        if (a.bias != nullptr && block < last_blocks) {
+          bias[i][0] = bias_at(a, col + lane);
+          bias[i][1] = bias_at(a, col + 32 + lane);
+        }
+      }
       if (!ptx::mbar_wait_warp(acc_full + acc, acc_phase)) {
         atomicExch(&g_linear_status, kLinEpilogue);
+        linger();
         break;
       }
       ptx::tc_fence_after();
-      uint32_t r[2][32];
-      const uint32_t src = tmem + ((uint32_t)quarter << 21) + acc * C::kTileN + group * 64;
-      ptx::tc_ld_32x32(src, r[0]);
-      ptx::tc_ld_32x32(src + 32, r[1]);
+      uint32_t r[2][2][32];              // (columns past the tile hold whatever they hold and are not used)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t src = tmem + ((uint32_t)quarter << 21) + acc * C::kTileN + (group + 2 * i) * 64;
+        ptx::tc_ld_32x32(src, r[i][0]);
+        ptx::tc_ld_32x32(src + 32, r[i][1]);
+      }
       ptx::tc_ld_wait();
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive_cluster(acc_empty + acc, 0);
       if (++acc == C::kAccs) { acc = 0; acc_phase ^= 1; }
-      const int row = mt * 256 + (int)rank * 128 + quarter * 32 + lane;
-      const int col = nt * 256 + group * 64;
-      const bool live = row < a.rows && col < a.features;
-      if (live && a.gated) {
 #pragma unroll
-        for (int h = 0; h < 32; h += 16) {
-          float g[16], u[16], y[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) { g[j] = __uint_as_float(r[0][h + j]); u[j] = __uint_as_float(r[1][h + j]); }
-          add_bias(g, a, col + h);
-          add_bias(u, a, col + 32 + h);
-          gate(g, u, y, a);
-          store_outputs(y, a, row, col / 2 + h);
+      for (int i = 0; i < 2; ++i) {
+        const int block = group + 2 * i, col = nt * a.tile_n + block * 64, out_col = a.gated ? col / 2 : col;
+        if (!ok || block >= last_blocks) continue;
+        // features of the block that belong to the tile (a multiple of 32) and to the matrix
+        const int width = min(min(64, a.tile_n - block * 64), a.features - col);
+        if (staged_res) {
+          if (!ptx::mbar_wait_warp(res_full + warp - 2, res_phase)) {
+            atomicExch(&g_linear_status, kLinResidual);
+            linger();
+            ok = false;
+            continue;
+          }
+          res_phase ^= 1;
+        } else if (a.tma_out) {
+          if (lane == 0) ptx::bulk_wait_read_all();
+          __syncwarp();
         }
-      } else if (live) {
+        if (a.bias != nullptr) {
 #pragma unroll
-        for (int h = 0; h < 64; h += 16) {
-          if (col + h < a.features) {
-            float v[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[h / 32][h % 32 + j]);
-            add_bias(v, a, col + h);
-            activate(v, a);
-            store_outputs(v, a, row, col + h);
+          for (int j = 0; j < 32; ++j) {
+            r[i][0][j] = __float_as_uint(__uint_as_float(r[i][0][j]) + __shfl_sync(0xffffffffu, bias[i][0], j));
+            r[i][1][j] = __float_as_uint(__uint_as_float(r[i][1][j]) + __shfl_sync(0xffffffffu, bias[i][1], j));
           }
         }
+#pragma unroll
+        for (int h = 0; h < 64; h += 16) {
+          if (a.gated ? h >= 32 || 2 * h >= width : h >= width) continue;      // (gated: a whole block or nothing)
+          float v[16];
+          if (a.gated) {
+            if (h < 32) {
+              float g[16], u[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) { g[j] = __uint_as_float(r[i][0][h % 32 + j]); u[j] = __uint_as_float(r[i][1][h % 32 + j]); }
+              gate(g, u, v, a);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[i][h / 32][h % 32 + j]);
+            activate(v, a);
+          }
+          // this thread's row of the box, 16-byte pieces swizzled by the row
+          uint4* line = reinterpret_cast<uint4*>(mine + (h / 32) * 2048 + lane * 64);
+          const int swz = (lane >> 1) & 3, piece = (h % 32) / 8;
+          if (staged_res) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float f[8];
+              unpack8(line[(piece + j) ^ swz], f);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) v[8 * j + q] += f[q];
+            }
+          }
+          if (a.tma_out) {
+            if (!staged_res && a.residual != nullptr && row < a.rows) add_residual(v, a, row, out_col + h);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              line[(piece + j) ^ swz] = make_uint4(as_u32(__floats2bfloat162_rn(v[8 * j], v[8 * j + 1])), as_u32(__floats2bfloat162_rn(v[8 * j + 2], v[8 * j + 3])),
+                                                   as_u32(__floats2bfloat162_rn(v[8 * j + 4], v[8 * j + 5])), as_u32(__floats2bfloat162_rn(v[8 * j + 6], v[8 * j + 7])));
+          } else if (row < a.rows) {
+            if (!staged_res) add_residual(v, a, row, out_col + h);
+            store_outputs(v, a, row, out_col + h);
+          }
+        }
+        if (a.tma_out) ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (a.tma_out && row0 < a.rows && width > 0) {
+            ptx::tma_store_3d(&map_out, mine, out_col, row0, 0);
+            if (!a.gated && width > 32) ptx::tma_store_3d(&map_out, mine + 2048, out_col + 32, row0, 0);
+            ptx::bulk_commit();
+          }
+          if (staged_res) {              // the next block's residual, once the copies have read this one's outputs
+            ptx::bulk_wait_read_all();
+            if (block + 2 < last_blocks) {
+              ask(row0, nt, block + 2);
+            } else if (tile + pairs < tiles) {
+              int mt2, nt2;
+              pair_tile(tile + pairs, a.m_tiles, a.n_tiles, mt2, nt2);
+              ask(mt2 * 256 + (int)rank * 128 + quarter * 32, nt2, group);
+            }
+          }
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
+    if (lane == 0) ptx::bulk_wait_all();
   }
   __syncwarp();
   ptx::tc_fence_before();
@@ -729,6 +839,25 @@ int scale_map(CUtensorMap* map, const void* base, uint64_t row_atoms, uint64_t k
   });
 }
 
+// bf16 rows [rows][width], `stride` elements apart, in boxes of 32 x 32 (64-byte swizzle): outputs and residuals.
+int rows_map(CUtensorMap* map, const void* base, uint64_t width, uint64_t rows, uint64_t stride) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  return cached_map(g_linear_maps, map, MapKey{base, width, rows, stride, 32, 32, 2u}, [&](CUtensorMap* m) {
+    cuuint64_t dims[3] = {width, rows, 1};
+    cuuint64_t strides[2] = {stride * 2, stride * 2 * rows};
+    cuuint32_t box[3] = {32, 32, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+      return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled (rows) failed with CUresult %d (width=%llu rows=%llu)", (int)r,
+                  (unsigned long long)width, (unsigned long long)rows);
+    return (int)PNV_OK;
+  });
+}
+
+constexpr int kFill = 64;                // bytes a CTA takes in from L2 in a cycle
 constexpr int kMaxSplitLog = 3;          // clusters of 1, 2, 4 or 8 CTAs
 
 // Per kernel and device, once: shared-memory carve-out, and how many clusters of each size run at one time.
@@ -818,18 +947,24 @@ int launch_split(const Operands& o, const LinearArgs& a, int split, cudaStream_t
 }
 
 template <bool kMx8>
-int launch_pair(const Operands& o, const LinearArgs& a, int pairs, cudaStream_t stream) {
+int launch_pair(const Operands& o, LinearArgs a, int pairs, cudaStream_t stream) {
   using C = PairCfg<kMx8>;
-  CUtensorMap map_w, map_x, map_w_sf = {}, map_x_sf = {};
-  if (int rc = operand_map(&map_w, o.w, a.k_bytes, a.features, a.k_bytes, 128)) return rc;
+  CUtensorMap map_w, map_x, map_w_sf = {}, map_x_sf = {}, map_out = {}, map_res = {};
+  if (int rc = operand_map(&map_w, o.w, a.k_bytes, a.features, a.k_bytes, a.tile_n / 2)) return rc;
   if (int rc = operand_map(&map_x, o.x, a.k_bytes, a.rows, o.x_stride, 128)) return rc;
   if (kMx8) {
     const int k_atoms = ceil_div_i(a.k_bytes, 128);
     if (int rc = scale_map(&map_w_sf, a.w_sf, sf_row_atoms(a.features), k_atoms, 2)) return rc;
     if (int rc = scale_map(&map_x_sf, a.x_sf, sf_row_atoms(a.rows), k_atoms, 1)) return rc;
   }
+  a.tma_out = a.vec_out;
+  a.tma_res = a.tma_out && a.residual != nullptr && a.vec_residual;
+  if (a.tma_out)
+    if (int rc = rows_map(&map_out, a.out, a.n_out, a.rows, a.n_out)) return rc;
+  if (a.tma_res)
+    if (int rc = rows_map(&map_res, a.residual, a.n_out, a.rows, a.residual_stride)) return rc;
   PNV_CUDA(launch_clusters(linear_pair_kernel<kMx8>, dim3((unsigned)(2 * pairs)), C::kThreads, C::kSmem, 2, stream, map_w, map_x, map_w_sf,
-                           map_x_sf, a));
+                           map_x_sf, map_out, map_res, a));
   return PNV_OK;
 }
 
@@ -850,15 +985,24 @@ int run_linear(const Operands& o, LinearArgs a, int sm_count, cudaStream_t strea
     const int* pair_clusters = nullptr;
     if (int rc = pair_setup<kMx8>(&pair_clusters)) return rc;
     const int pairs = std::min(pair_clusters[1], sm_count / 2);
-    const long long m_tiles = ceil_div_i(a.rows, 256), n_tiles = ceil_div_i(a.features, 256), pair_tiles = m_tiles * n_tiles;
-    // A stage of a 128 x 128 tile and one of a 256 x 256 tile of a pair take about as long: both are bound by what a CTA
-    // takes in from L2, which is the same 32 KB.
-    const long long split_waves = (tiles * split + sm_count - 1) / sm_count;
-    if (pairs >= 1 && pair_tiles < (1LL << 31) / kBand && (pair_tiles + pairs - 1) / pairs * split <= split_waves) {
-      a.m_tiles = (int)m_tiles;
-      a.n_tiles = (int)n_tiles;
-      return launch_pair<kMx8>(o, a, (int)std::min<long long>(pairs, pair_tiles), stream);
+    const long long m_tiles = ceil_div_i(a.rows, 256);
+    // Cycles of a stage: the products of a pair's tile, 2 per feature, or what a CTA takes in, 64 bytes a cycle, whichever is
+    // more.  (Widths: of 32 features; of 64 where the scales' atoms or the gates' blocks ask for it.)
+    const int step = kMx8 || a.gated ? 64 : 32;
+    long long best = 0;
+    for (int width = 256; pairs >= 1 && width >= 128; width -= step) {
+      const long long tiles_n = ceil_div_i(a.features, width), waves = (m_tiles * tiles_n + pairs - 1) / pairs;
+      const long long cost = waves * std::max(2 * width, (kABytes + width / 2 * kStageRow) / kFill);
+      if (m_tiles * tiles_n < (1LL << 31) / kBand && (best == 0 || cost < best)) {
+        best = cost;
+        a.m_tiles = (int)m_tiles;
+        a.n_tiles = (int)tiles_n;
+        a.tile_n = width;
+      }
     }
+    const long long split_waves = (tiles * split + sm_count - 1) / sm_count;
+    if (best > 0 && best * split <= split_waves * ((kABytes + 128 * kStageRow) / kFill))
+      return launch_pair<kMx8>(o, a, (int)std::min<long long>(pairs, m_tiles * a.n_tiles), stream);
   }
   PNV_REQUIRE(ceil_div_i(a.rows, bn) <= 65535 && ceil_div_i(a.features, kTileRows) < (1 << 28), "linear: too many rows for one call");
   switch (bn) {
@@ -911,11 +1055,10 @@ int linear_common(bool mx8, void* out, int out_is_f32, const void* x, long long 
   a.bias_f32 = bias_is_f32;
   a.gated = gated;
   a.kind = act_kind;
-  // (pieces of a row start at multiples of 8 outputs, those of the pair kernel at multiples of 16)
-  const int out_pitch = n_out * (out_is_f32 ? 4 : 2);
-  a.vec_out = out_pitch % 32 == 0 && at(out, 32) ? 32 : out_pitch % 16 == 0 && at(out, 16) ? 16 : 0;
-  a.vec_residual = residual_stride % 8 == 0 && at(residual, 16) ? 16 : 0;
-  a.vec_bias = at(bias, 16) ? 16 : 0;
+  // (pieces of a row start at multiples of 8 outputs)
+  a.vec_out = n_out * (out_is_f32 ? 4 : 2) % 16 == 0 && at(out, 16);
+  a.vec_residual = residual_stride % 8 == 0 && at(residual, 16);
+  a.vec_bias = at(bias, 16);
   if (sm_count <= 0) sm_count = 148;
   const Operands o{x, w, stride_bytes};
   return mx8 ? run_linear<true>(o, a, sm_count, stream) : run_linear<false>(o, a, sm_count, stream);

@@ -382,11 +382,10 @@ __device__ __forceinline__ void tc_mma_mxf8(uint32_t d_tmem, uint64_t a_desc, ui
                  "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
                  :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem) : "memory");
 }
-// A / B format (e4m3 = 0), scale byte of B bits 4-5, N/8 bits 17-22, scale format (1 = UE8M0) bit 23, M/16 bits 24-28, scale
-// byte of A bits 29-30.
-__host__ __device__ constexpr uint32_t mma_mxf8_idesc(int n, int m, int scale_byte) {
-  return ((uint32_t)scale_byte << 4) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) | ((uint32_t)scale_byte << 29);
-}
+// A / B format (e4m3 = 0), N/8 bits 17-22, scale format (1 = UE8M0) bit 23, M/16 bits 24-28; the byte of the scale words: of B
+// bits 4-5, of A bits 29-30.
+__host__ __device__ constexpr uint32_t mma_mxf8_idesc(int n, int m) { return ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24); }
+__host__ __device__ constexpr uint32_t mma_mxf8_scale_byte(int i) { return ((uint32_t)i << 4) | ((uint32_t)i << 29); }
 
 // The matrix-fragment form: 16 lanes x 8 columns per step (16x256b), 4 or 2 steps.  Of step j a thread gets
 // r[4j], r[4j+1] = (lane l / 4, columns 8j + 2 (l % 4) and the next one) and r[4j+2], r[4j+3] = the same columns eight
