@@ -55,6 +55,10 @@ struct LinearArgs {
   int tma_out, tma_res;                  // pair kernel: do outputs leave and residuals come by TMA copies
 };
 
+// What an epilogue does between bias and residual.  Kernels are compiled for each: with all the activations' code in one
+// epilogue, jumped over four times a block, a block of 64 features took 2200 cycles where nothing was to be activated.
+enum Mode : int { kNothing = 0, kActivate = 1, kGate = 2 };
+
 // ---- epilogue arithmetic -------------------------------------------------------------------------
 
 __device__ __forceinline__ float silu_f32(float g) { return g * rcp_approx(1.f + ex2_approx(g * -kLog2e)); }
@@ -246,7 +250,7 @@ struct SplitCfg {
   static_assert(kColsUsed <= 512 && kStages > kIssuers, "tensor-memory column map or pipeline");
 };
 
-template <int BN, bool kMx8>
+template <int BN, bool kMx8, int kMode>
 __global__ void __launch_bounds__(SplitCfg<BN, kMx8>::kThreads, 1)
 linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LinearArgs a,
                     const int split) {
@@ -448,11 +452,11 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   }
 
   // ---- this CTA's share of the tile's outputs, in pieces of eight neighbouring features of a token
-  const int per_token = a.gated ? 8 : 16;
+  const int per_token = kMode == kGate ? 8 : 16;
   for (int u = (int)threadIdx.x; u < own * per_token; u += C::kThreads) {
     const int token = u / per_token, piece = u - token * per_token;
     // gated: features [64 b, 64 b + 32) are gates, the next 32 their ups
-    const int f = a.gated ? (piece >> 2) * 64 + (piece & 3) * 8 : piece * 8;
+    const int f = kMode == kGate ? (piece >> 2) * 64 + (piece & 3) * 8 : piece * 8;
     const int col = ft * kTileRows + f, row = tt * BN + rank * share + token;
     if (col >= a.features) continue;
     float v[8], up[8];
@@ -464,14 +468,14 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       const float4 p = src[0], q = src[1];
       v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
       v[4] += q.x; v[5] += q.y; v[6] += q.z; v[7] += q.w;
-      if (a.gated) {
+      if constexpr (kMode == kGate) {
         const float4 s = src[8], t = src[9];
         up[0] += s.x; up[1] += s.y; up[2] += s.z; up[3] += s.w;
         up[4] += t.x; up[5] += t.y; up[6] += t.z; up[7] += t.w;
       }
     }
     add_bias(v, a, col);
-    if (a.gated) {
+    if constexpr (kMode == kGate) {
       add_bias(up, a, col + 32);
       float y[8];
       gate(v, up, y, a);
@@ -479,7 +483,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       add_residual(y, a, row, out_col);
       store_outputs(y, a, row, out_col);
     } else {
-      activate(v, a);
+      if constexpr (kMode == kActivate) activate(v, a);
       add_residual(v, a, row, col);
       store_outputs(v, a, row, col);
     }
@@ -524,7 +528,7 @@ __device__ __forceinline__ int tile_nt(int tile, const LinearArgs& a) {
   return nt;
 }
 
-template <bool kMx8>
+template <bool kMx8, int kMode>
 __global__ void __launch_bounds__(PairCfg<kMx8>::kThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const __grid_constant__ CUtensorMap map_w_sf, const __grid_constant__ CUtensorMap map_x_sf,
@@ -656,10 +660,10 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     bool ok = true;
     // The residual of a block of a tile (tokens from row0 on) is asked for; lane 0, whose stores from there have been read.
     auto ask = [&](int row0, int nt, int block) {
-      const int col = nt * a.tile_n + block * 64, out0 = a.gated ? col / 2 : col;
-      ptx::mbar_arrive_expect_tx(res_full + warp - 2, a.gated ? 2048 : 4096);
+      const int col = nt * a.tile_n + block * 64, out0 = kMode == kGate ? col / 2 : col;
+      ptx::mbar_arrive_expect_tx(res_full + warp - 2, kMode == kGate ? 2048 : 4096);
       ptx::tma_load_3d(mine, &map_res, res_full + warp - 2, out0, row0, 0);
-      if (!a.gated) ptx::tma_load_3d(mine + 2048, &map_res, res_full + warp - 2, out0 + 32, row0, 0);
+      if (kMode != kGate) ptx::tma_load_3d(mine + 2048, &map_res, res_full + warp - 2, out0 + 32, row0, 0);
     };
     const int last_blocks = (a.tile_n + 63) / 64;
     if (staged_res && group < last_blocks && (int)blockIdx.x / 2 < tiles && lane == 0) {
@@ -703,7 +707,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       if (++acc == C::kAccs) { acc = 0; acc_phase ^= 1; }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int block = group + 2 * i, col = nt * a.tile_n + block * 64, out_col = a.gated ? col / 2 : col;
+        const int block = group + 2 * i, col = nt * a.tile_n + block * 64, out_col = kMode == kGate ? col / 2 : col;
         if (!ok || block >= last_blocks) continue;
         // features of the block that belong to the tile (a multiple of 32) and to the matrix
         const int width = min(min(64, a.tile_n - block * 64), a.features - col);
@@ -728,9 +732,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         }
 #pragma unroll
         for (int h = 0; h < 64; h += 16) {
-          if (a.gated ? h >= 32 || 2 * h >= width : h >= width) continue;      // (gated: a whole block or nothing)
+          if (kMode == kGate ? h >= 32 || 2 * h >= width : h >= width) continue;      // (gated: a whole block or nothing)
           float v[16];
-          if (a.gated) {
+          if constexpr (kMode == kGate) {
             if (h < 32) {
               float g[16], u[16];
 #pragma unroll
@@ -740,7 +744,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
           } else {
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[i][h / 32][h % 32 + j]);
-            activate(v, a);
+            if constexpr (kMode == kActivate) activate(v, a);
           }
           // this thread's row of the box, 16-byte pieces swizzled by the row
           uint4* line = reinterpret_cast<uint4*>(mine + (h / 32) * 2048 + lane * 64);
@@ -770,7 +774,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         if (lane == 0) {
           if (a.tma_out && row0 < a.rows && width > 0) {
             ptx::tma_store_3d(&map_out, mine, out_col, row0, 0);
-            if (!a.gated && width > 32) ptx::tma_store_3d(&map_out, mine + 2048, out_col + 32, row0, 0);
+            if (kMode != kGate && width > 32) ptx::tma_store_3d(&map_out, mine + 2048, out_col + 32, row0, 0);
             ptx::bulk_commit();
           }
           if (staged_res) {              // the next block's residual, once the copies have read this one's outputs
@@ -924,29 +928,29 @@ struct Operands {
   long long x_stride;                    // bytes
 };
 
-template <int BN, bool kMx8>
+template <int BN, bool kMx8, int kMode>
 int split_setup(const int** clusters) {
   static Setup setup;
-  return prepare(linear_split_kernel<BN, kMx8>, setup, SplitCfg<BN, kMx8>::kThreads, SplitCfg<BN, kMx8>::kSmem, clusters);
+  return prepare(linear_split_kernel<BN, kMx8, kMode>, setup, SplitCfg<BN, kMx8>::kThreads, SplitCfg<BN, kMx8>::kSmem, clusters);
 }
-template <bool kMx8>
+template <bool kMx8, int kMode>
 int pair_setup(const int** clusters) {
   static Setup setup;
-  return prepare(linear_pair_kernel<kMx8>, setup, PairCfg<kMx8>::kThreads, PairCfg<kMx8>::kSmem, clusters);
+  return prepare(linear_pair_kernel<kMx8, kMode>, setup, PairCfg<kMx8>::kThreads, PairCfg<kMx8>::kSmem, clusters);
 }
 
-template <int BN, bool kMx8>
+template <int BN, bool kMx8, int kMode>
 int launch_split(const Operands& o, const LinearArgs& a, int split, cudaStream_t stream) {
   using C = SplitCfg<BN, kMx8>;
   CUtensorMap map_w, map_x;
   if (int rc = operand_map(&map_w, o.w, a.k_bytes, a.features, a.k_bytes, kTileRows)) return rc;
   if (int rc = operand_map(&map_x, o.x, a.k_bytes, a.rows, o.x_stride, BN)) return rc;
   const dim3 grid((unsigned)(ceil_div_i(a.features, kTileRows) * split), (unsigned)ceil_div_i(a.rows, BN));
-  PNV_CUDA(launch_clusters(linear_split_kernel<BN, kMx8>, grid, C::kThreads, C::kSmem, split, stream, map_w, map_x, a, split));
+  PNV_CUDA(launch_clusters(linear_split_kernel<BN, kMx8, kMode>, grid, C::kThreads, C::kSmem, split, stream, map_w, map_x, a, split));
   return PNV_OK;
 }
 
-template <bool kMx8>
+template <bool kMx8, int kMode>
 int launch_pair(const Operands& o, LinearArgs a, int pairs, cudaStream_t stream) {
   using C = PairCfg<kMx8>;
   CUtensorMap map_w, map_x, map_w_sf = {}, map_x_sf = {}, map_out = {}, map_res = {};
@@ -963,27 +967,27 @@ int launch_pair(const Operands& o, LinearArgs a, int pairs, cudaStream_t stream)
     if (int rc = rows_map(&map_out, a.out, a.n_out, a.rows, a.n_out)) return rc;
   if (a.tma_res)
     if (int rc = rows_map(&map_res, a.residual, a.n_out, a.rows, a.residual_stride)) return rc;
-  PNV_CUDA(launch_clusters(linear_pair_kernel<kMx8>, dim3((unsigned)(2 * pairs)), C::kThreads, C::kSmem, 2, stream, map_w, map_x, map_w_sf,
+  PNV_CUDA(launch_clusters(linear_pair_kernel<kMx8, kMode>, dim3((unsigned)(2 * pairs)), C::kThreads, C::kSmem, 2, stream, map_w, map_x, map_w_sf,
                            map_x_sf, map_out, map_res, a));
   return PNV_OK;
 }
 
 // Which kernel, and how many CTAs share a tile's K.
-template <bool kMx8>
+template <bool kMx8, int kMode>
 int run_linear(const Operands& o, LinearArgs a, int sm_count, cudaStream_t stream) {
   const int k_stages = ceil_div_i(a.k_bytes, kStageRow);
   const int bn = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : a.rows <= 64 ? 64 : 128;
   const long long tiles = (long long)ceil_div_i(a.features, kTileRows) * ceil_div_i(a.rows, bn);
   const int* clusters = nullptr;
-  if (int rc = bn == 16 ? split_setup<16, kMx8>(&clusters) : bn == 32 ? split_setup<32, kMx8>(&clusters)
-             : bn == 64 ? split_setup<64, kMx8>(&clusters) : split_setup<128, kMx8>(&clusters))
+  if (int rc = bn == 16 ? split_setup<16, kMx8, kMode>(&clusters) : bn == 32 ? split_setup<32, kMx8, kMode>(&clusters)
+             : bn == 64 ? split_setup<64, kMx8, kMode>(&clusters) : split_setup<128, kMx8, kMode>(&clusters))
     return rc;
   int split = 1;
   for (int i = 1; i <= kMaxSplitLog; ++i)
     if (tiles <= std::min(clusters[i], sm_count >> i) && (k_stages >> i) >= 2) split = 1 << i;
   if (!a.out_f32 && bn == 128) {
     const int* pair_clusters = nullptr;
-    if (int rc = pair_setup<kMx8>(&pair_clusters)) return rc;
+    if (int rc = pair_setup<kMx8, kMode>(&pair_clusters)) return rc;
     const int pairs = std::min(pair_clusters[1], sm_count / 2);
     const long long m_tiles = ceil_div_i(a.rows, 256);
     // Cycles of a stage: the products of a pair's tile, 2 per feature, or what a CTA takes in, 64 bytes a cycle, whichever is
@@ -1002,14 +1006,14 @@ int run_linear(const Operands& o, LinearArgs a, int sm_count, cudaStream_t strea
     }
     const long long split_waves = (tiles * split + sm_count - 1) / sm_count;
     if (best > 0 && best * split <= split_waves * ((kABytes + 128 * kStageRow) / kFill))
-      return launch_pair<kMx8>(o, a, (int)std::min<long long>(pairs, m_tiles * a.n_tiles), stream);
+      return launch_pair<kMx8, kMode>(o, a, (int)std::min<long long>(pairs, m_tiles * a.n_tiles), stream);
   }
   PNV_REQUIRE(ceil_div_i(a.rows, bn) <= 65535 && ceil_div_i(a.features, kTileRows) < (1 << 28), "linear: too many rows for one call");
   switch (bn) {
-    case 16: return launch_split<16, kMx8>(o, a, split, stream);
-    case 32: return launch_split<32, kMx8>(o, a, split, stream);
-    case 64: return launch_split<64, kMx8>(o, a, split, stream);
-    default: return launch_split<128, kMx8>(o, a, split, stream);
+    case 16: return launch_split<16, kMx8, kMode>(o, a, split, stream);
+    case 32: return launch_split<32, kMx8, kMode>(o, a, split, stream);
+    case 64: return launch_split<64, kMx8, kMode>(o, a, split, stream);
+    default: return launch_split<128, kMx8, kMode>(o, a, split, stream);
   }
 }
 
@@ -1061,7 +1065,10 @@ int linear_common(bool mx8, void* out, int out_is_f32, const void* x, long long 
   a.vec_bias = at(bias, 16);
   if (sm_count <= 0) sm_count = 148;
   const Operands o{x, w, stride_bytes};
-  return mx8 ? run_linear<true>(o, a, sm_count, stream) : run_linear<false>(o, a, sm_count, stream);
+  if (gated) return mx8 ? run_linear<true, kGate>(o, a, sm_count, stream) : run_linear<false, kGate>(o, a, sm_count, stream);
+  if (act_kind != PNV_ACT_NONE)
+    return mx8 ? run_linear<true, kActivate>(o, a, sm_count, stream) : run_linear<false, kActivate>(o, a, sm_count, stream);
+  return mx8 ? run_linear<true, kNothing>(o, a, sm_count, stream) : run_linear<false, kNothing>(o, a, sm_count, stream);
 }
 
 }  // namespace
