@@ -9,6 +9,7 @@
 // so two that lie closer together than those can be off might come out in the wrong order: where a selected key is that
 // close to the next one, the row is done again in 64 bits (a handful of rows in a thousand at 256 experts).
 // Bound: latency of the reductions for few rows, issue slots for many.
+#include <algorithm>
 #include <climits>
 
 #include "common.cuh"
@@ -16,7 +17,8 @@
 namespace pnv {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;                // of a block
+constexpr int kBlocks = 8;               // of an SM at most: further rows are walked over
 constexpr unsigned kAll = 0xffffffffu;
 
 struct RouteArgs {
@@ -83,20 +85,22 @@ __device__ __forceinline__ F softmax_sum(const RouteArgs& a, const void* row, in
   return sum;
 }
 
-// Are two neighbouring keys, the larger one first, too close for 32 bits to order?  A score is off by at most 1.5e-6 (a softmax over 1024), its sum
-// with the bias by half a unit more; a group's sum of two by twice that.
-__device__ __forceinline__ bool too_close(float larger, float smaller, float terms) {
-  return larger - smaller <= terms * 3.8146973e-6f * (1.f + fabsf(larger));
+// Are two neighbouring keys, the larger one first, too close for 32 bits to order?  A sigmoid is off by at most 2e-7 (2^-22 of
+// the exponential, times s (1 - s), and the reciprocal's unit), a softmax by 1.5e-6 (its sum over 1024), the sum with the bias
+// by half a unit more; a group's sum of two by twice that.
+__device__ __forceinline__ bool too_close(float larger, float smaller, float terms, bool sigmoid) {
+  return larger - smaller <= terms * (sigmoid ? 9.5367432e-7f : 3.8146973e-6f) * (1.f + fabsf(larger));
 }
 
-// Lane r < topk returns expert r of the row, best first.  doubtful: (32 bits with a bias) the order is not certain.
-template <class F, class O, int VPL>
-__device__ __forceinline__ int select(const RouteArgs& a, const void* row, int lane, bool& doubtful) {
-  const bool check = sizeof(F) == 4 && a.bias != nullptr;
+// Lane r < topk returns expert r of the row, best first, and its key; logit[j] is that of expert 32 j + lane.  doubtful: (32 bits
+// with a bias) the order is not certain.
+template <class F, class O, int VPL, bool kBias, bool kGroups>
+__device__ __forceinline__ int select(const RouteArgs& a, const void* row, const float (&logit)[VPL], int lane, O& picked_key, bool& doubtful) {
+  constexpr bool kCheck = kBias && sizeof(F) == 4;
   O key[VPL];
   {
     F mx = 0, total = 1;
-    if (a.bias != nullptr && !a.sigmoid) {
+    if (kBias && !a.sigmoid) {
       mx = (F)row_max(a, row, lane);
       total = softmax_sum<F>(a, row, lane, mx);
     }
@@ -105,120 +109,199 @@ __device__ __forceinline__ int select(const RouteArgs& a, const void* row, int l
       const int e = j * 32 + lane;
       key[j] = 0;
       if (e < a.experts) {
-        F k = (F)logit_at(a, row, e);
-        if (a.bias != nullptr) k = (a.sigmoid ? sigmoid_of(k) : softmax_part(k, mx) / total) + (F)__ldg(a.bias + e);
+        F k = (F)logit[j];
+        if (kBias) k = (a.sigmoid ? sigmoid_of(k) : softmax_part(k, mx) / total) + (F)__ldg(a.bias + e);
         key[j] = order_of(k);
       }
     }
   }
   doubtful = false;
-  if (a.groups > 1) {
+  if constexpr (kGroups) {
     O mine = 0;                          // lane g: the score of group g
-    for (int g = 0; g < a.groups; ++g) {
-      O first = 0, second = 0;           // this lane's two best of the group
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        const bool in = (((unsigned)(j * 32 + lane) * a.group_inv) >> 20) == (unsigned)g;
-        const O k = in ? key[j] : (O)0;
-        second = max(second, min(first, k));
-        first = max(first, k);
-      }
+    int g = 0;
+    O first = 0, second = 0;             // this lane's two best of a group
+    auto take = [&](O k) {
+      if (kBias) second = max(second, min(first, k));
+      first = max(first, k);
+    };
+    auto close_group = [&]() {
       const O best = warp_max(first);
       O score = best;
-      if (a.bias != nullptr) {
+      if (kBias) {
         const int owner = __ffs(__ballot_sync(kAll, first == best)) - 1;
         const O next = warp_max(lane == owner ? second : first);
         score = next == 0 ? best : order_of(key_of(best) + key_of(next));
       }
       if (lane == g) mine = score;
+      first = second = 0;
+      ++g;
+    };
+    if (a.group_size % 32 == 0) {        // whole registers belong to a group
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        take(key[j]);
+        if ((j + 1) * 32 % a.group_size == 0 && g < a.groups) close_group();
+      }
+    } else {
+#pragma unroll 1
+      while (g < a.groups) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) take((((unsigned)(j * 32 + lane) * a.group_inv) >> 20) == (unsigned)g ? key[j] : (O)0);
+        close_group();
+      }
     }
     unsigned kept = 0;
     F last = 0;
+#pragma unroll 1
     for (int r = 0; r <= a.topk_groups && r < a.groups; ++r) {
       const O best = warp_max(mine);
-      const int g = __ffs(__ballot_sync(kAll, mine == best && lane < a.groups)) - 1;
-      const F k = key_of(best);
-      // (the order among the kept does not matter, only the border)
-      if (r == a.topk_groups) {
-        if (check) doubtful |= too_close((float)last, (float)k, 2.f);
+      if (r == a.topk_groups) {          // (the order among the kept does not matter, only the border)
+        if (kCheck) doubtful |= too_close((float)last, (float)key_of(best), 2.f, a.sigmoid);
         break;
       }
-      last = k;
-      kept |= 1u << g;
-      if (lane == g) mine = 0;
+      const int chosen = __ffs(__ballot_sync(kAll, mine == best && lane < a.groups)) - 1;
+      last = key_of(best);
+      kept |= 1u << chosen;
+      if (lane == chosen) mine = 0;
     }
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-      const unsigned g = ((unsigned)(j * 32 + lane) * a.group_inv) >> 20;
-      if (g >= 32 || !((kept >> g) & 1)) key[j] = 0;
+      const unsigned of = ((unsigned)(j * 32 + lane) * a.group_inv) >> 20;
+      if (of >= 32 || !((kept >> of) & 1)) key[j] = 0;
     }
   }
+  // Up to eight keys a lane are sorted first (equal ones in the order of their experts): a round then looks at one key a lane,
+  // and the lane that had the best one moves up.
+  constexpr bool kSorted = VPL <= 8;
+  int expert[VPL];
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) expert[j] = j * 32 + lane;
+  if constexpr (kSorted) {
+#pragma unroll
+    for (int i = 1; i < VPL; ++i)
+#pragma unroll
+      for (int j = i; j > 0; --j) {
+        const bool swap = key[j] > key[j - 1];
+        const O hi = swap ? key[j] : key[j - 1], lo = swap ? key[j - 1] : key[j];
+        const int he = swap ? expert[j] : expert[j - 1], le = swap ? expert[j - 1] : expert[j];
+        key[j - 1] = hi; key[j] = lo;
+        expert[j - 1] = he; expert[j] = le;
+      }
+  }
   int picked = 0;
+  picked_key = 0;
   F last = 0;
-  const int rounds = check ? a.topk + 1 : a.topk;         // one more to see how close the next one is
+  const int rounds = kCheck ? a.topk + 1 : a.topk;        // one more to see how close the next one is
+#pragma unroll 1
   for (int r = 0; r < rounds; ++r) {
     O first = key[0];
+    int mine = expert[0];
+    if constexpr (!kSorted) {
 #pragma unroll
-    for (int j = 1; j < VPL; ++j) first = max(first, key[j]);
+      for (int j = 1; j < VPL; ++j)
+        if (key[j] > first) { first = key[j]; mine = expert[j]; }
+    }
     const O best = warp_max(first);
-    if (best == 0) break;                // (only the round beyond the last: there are topk experts to choose from)
-    int e = INT_MAX;
+    if (kCheck && best == 0) break;      // (only the round beyond the last: there are topk experts to choose from)
+    const unsigned with = __ballot_sync(kAll, first == best);
+    int e = __shfl_sync(kAll, mine, __ffs(with) - 1);
+    if (with & (with - 1)) e = __reduce_min_sync(kAll, first == best ? mine : INT_MAX);
+    if constexpr (kSorted) {
+      if (mine == e) {
 #pragma unroll
-    for (int j = VPL - 1; j >= 0; --j)
-      if (key[j] == best) e = j * 32 + lane;
-    e = __reduce_min_sync(kAll, e);
+        for (int j = 0; j + 1 < VPL; ++j) { key[j] = key[j + 1]; expert[j] = expert[j + 1]; }
+        key[VPL - 1] = 0;
+      }
+    } else {
 #pragma unroll
-    for (int j = 0; j < VPL; ++j)
-      if (e == j * 32 + lane) key[j] = 0;
-    if (check) {
+      for (int j = 0; j < VPL; ++j)
+        if (expert[j] == e) key[j] = 0;
+    }
+    if (kCheck) {
       const F k = key_of(best);
-      if (r > 0) doubtful |= too_close((float)last, (float)k, 1.f);
+      if (r > 0) doubtful |= too_close((float)last, (float)k, 1.f, a.sigmoid);
       last = k;
     }
-    if (lane == r) picked = e;
+    if (lane == r) { picked = e; picked_key = best; }
   }
   return picked;
 }
 
 template <int VPL>
-__device__ __noinline__ int select_exactly(const RouteArgs& a, const void* row, int lane) {
-  bool ignored;
-  return select<double, unsigned long long, VPL>(a, row, lane, ignored);
+__device__ __forceinline__ void load_row(const RouteArgs& a, const void* row, int lane, float (&logit)[VPL]) {
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) logit[j] = j * 32 + lane < a.experts ? logit_at(a, row, j * 32 + lane) : 0.f;
 }
 
-template <int VPL>
+template <int VPL, bool kGroups>
+__device__ __noinline__ int select_exactly(const RouteArgs& a, const void* row, int lane) {
+  float logit[VPL];
+  load_row(a, row, lane, logit);
+  bool ignored;
+  unsigned long long key;
+  return select<double, unsigned long long, VPL, true, kGroups>(a, row, logit, lane, key, ignored);
+}
+
+template <int VPL, bool kBias, bool kGroups>
 __global__ void __launch_bounds__(kWarps * 32)
 route_topk_kernel(const RouteArgs a) {
   pdl_wait();
   pdl_launch_dependents();
-  const long long t = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (t >= a.rows) return;
-  const void* row = static_cast<const uint8_t*>(a.logits) + t * a.stride * (a.bf16 ? 2 : 4);
-  bool doubtful;
-  int e = select<float, uint32_t, VPL>(a, row, lane, doubtful);
-  if (doubtful) e = select_exactly<VPL>(a, row, lane);
-  float w = 0.f;
-  if (a.sigmoid) {
-    if (lane < a.topk) w = __fdiv_rn(1.f, 1.f + expf(-logit_at(a, row, e)));
-  } else {
-    const float mx = row_max(a, row, lane);
-    if (lane < a.topk) w = softmax_part(logit_at(a, row, e), mx);
-    if (!a.renormalize) {
-      const float total = softmax_sum<float>(a, row, lane, mx);
-      w = total > 0.f ? __fdiv_rn(w, total) : total;               // (a NaN stays one)
+  const long long step = (long long)gridDim.x * kWarps;
+  const long long row_bytes = a.stride * (a.bf16 ? 2 : 4);
+  long long t = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  float logit[VPL], next[VPL];
+  if (t < a.rows) load_row(a, static_cast<const uint8_t*>(a.logits) + t * row_bytes, lane, next);
+  for (; t < a.rows; t += step) {
+    const uint8_t* row = static_cast<const uint8_t*>(a.logits) + t * row_bytes;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) logit[j] = next[j];
+    if (t + step < a.rows) load_row(a, row + step * row_bytes, lane, next);
+    bool doubtful;
+    uint32_t key;
+    int e = select<float, uint32_t, VPL, kBias, kGroups>(a, row, logit, lane, key, doubtful);
+    if constexpr (kBias) {
+      if (doubtful) e = select_exactly<VPL, kGroups>(a, row, lane);
+    }
+    float mine = 0.f;                    // the logit of this lane's choice: without a bias its key says it
+    if (lane < a.topk) mine = kBias ? logit_at(a, row, e) : key == 1u ? __uint_as_float(0x7FFFFFFFu) : key_of(key);
+    float w = 0.f;
+    if (a.sigmoid) {
+      if (lane < a.topk) w = __fdiv_rn(1.f, 1.f + expf(-mine));
+    } else {
+      float mx;                          // without bias and groups the first choice has it (a NaN is there only if all are)
+      if (!kBias && !kGroups) {
+        mx = __shfl_sync(kAll, mine, 0);
+        if (mx != mx) mx = -INFINITY;
+      } else {
+        mx = row_max(a, row, lane);
+      }
+      if (lane < a.topk) w = softmax_part(mine, mx);
+      if (!a.renormalize) {
+        const float total = softmax_sum<float>(a, row, lane, mx);
+        w = total > 0.f ? __fdiv_rn(w, total) : total;             // (a NaN stays one)
+      }
+    }
+    if (a.renormalize) {
+      float sum = w;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+      w = sum == 0.f ? 0.f : __fdiv_rn(w, sum);
+    }
+    if (lane < a.topk) {
+      a.ids[t * a.topk + lane] = e;
+      a.weights[t * a.topk + lane] = w * a.scale;
     }
   }
-  if (a.renormalize) {
-    float sum = w;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
-    w = sum == 0.f ? 0.f : __fdiv_rn(w, sum);
-  }
-  if (lane < a.topk) {
-    a.ids[t * a.topk + lane] = e;
-    a.weights[t * a.topk + lane] = w * a.scale;
-  }
+}
+
+using RouteKernel = void (*)(const RouteArgs);
+template <bool kBias, bool kGroups>
+RouteKernel route_kernel(int vpl) {
+  return vpl <= 1 ? route_topk_kernel<1, kBias, kGroups> : vpl <= 2 ? route_topk_kernel<2, kBias, kGroups>
+       : vpl <= 4 ? route_topk_kernel<4, kBias, kGroups> : vpl <= 8 ? route_topk_kernel<8, kBias, kGroups>
+       : vpl <= 16 ? route_topk_kernel<16, kBias, kGroups> : route_topk_kernel<32, kBias, kGroups>;
 }
 
 }  // namespace
@@ -228,7 +311,7 @@ using namespace pnv;
 
 extern "C" int pnv_route_topk(const void* logits, int logits_are_bf16, int64_t stride, int64_t rows, int experts, int topk, int sigmoid,
                               const float* bias, int groups, int topk_groups, int renormalize, float scale, float* weights,
-                              int32_t* ids, pnv_stream_t stream) {
+                              int32_t* ids, int sm_count, pnv_stream_t stream) {
   PNV_REQUIRE(rows >= 0 && rows < (1LL << 31), "bad row count");
   PNV_REQUIRE(experts >= 1 && experts <= PNV_ROUTE_MAX_EXPERTS, "route_topk: 1 to %d experts, got %d", PNV_ROUTE_MAX_EXPERTS, experts);
   PNV_REQUIRE(groups >= 1 && groups <= 32 && experts % groups == 0, "groups must divide the experts, at most 32, got %d", groups);
@@ -246,8 +329,9 @@ extern "C" int pnv_route_topk(const void* logits, int logits_are_bf16, int64_t s
   RouteArgs a{logits, bias, weights, (int*)ids, rows, stride, experts, topk, groups, topk_groups, group_size,
               (unsigned)(((1 << 20) + group_size - 1) / group_size), logits_are_bf16, sigmoid, renormalize, scale};
   const int vpl = ceil_div_i(experts, 32);
-  auto kernel = vpl <= 1 ? route_topk_kernel<1> : vpl <= 2 ? route_topk_kernel<2> : vpl <= 4 ? route_topk_kernel<4>
-              : vpl <= 8 ? route_topk_kernel<8> : vpl <= 16 ? route_topk_kernel<16> : route_topk_kernel<32>;
-  PNV_CUDA(launch_pdl(kernel, dim3((unsigned)((rows + kWarps - 1) / kWarps)), dim3(kWarps * 32), 0, (cudaStream_t)stream, pdl_enabled(), a));
+  const RouteKernel kernel = bias != nullptr ? groups > 1 ? route_kernel<true, true>(vpl) : route_kernel<true, false>(vpl)
+                                             : groups > 1 ? route_kernel<false, true>(vpl) : route_kernel<false, false>(vpl);
+  const long long blocks = std::min<long long>((rows + kWarps - 1) / kWarps, (long long)kBlocks * (sm_count > 0 ? sm_count : 148));
+  PNV_CUDA(launch_pdl(kernel, dim3((unsigned)blocks), dim3(kWarps * 32), 0, (cudaStream_t)stream, pdl_enabled(), a));
   return PNV_OK;
 }

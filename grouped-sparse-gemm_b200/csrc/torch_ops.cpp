@@ -791,7 +791,7 @@ std::tuple<Tensor, Tensor> route_topk(const Tensor& logits, int64_t topk, c10::s
   const c10::cuda::CUDAGuard guard(logits.device());
   check_rc(pnv_route_topk(logits.const_data_ptr(), is_bf16(logits) ? 1 : 0, row_stride(logits), T, (int)E, (int)topk, scoring == "sigmoid" ? 1 : 0,
                           bias.has_value() ? f32(*bias) : nullptr, (int)groups, (int)topk_groups, renormalize ? 1 : 0, (float)scale,
-                          weights.mutable_data_ptr<float>(), ids.mutable_data_ptr<int32_t>(), current_stream(logits)));
+                          weights.mutable_data_ptr<float>(), ids.mutable_data_ptr<int32_t>(), sm_count(logits), current_stream(logits)));
   return {weights, ids};
 }
 

@@ -367,7 +367,7 @@ int pnv_linear_device_status(int* status_out);
 #define PNV_ROUTE_MAX_EXPERTS 1024
 int pnv_route_topk(const void* logits, int logits_are_bf16, int64_t stride, int64_t rows, int experts, int topk, int sigmoid,
                    const float* bias, int groups, int topk_groups, int renormalize, float scale, float* weights,
-                   int32_t* ids, pnv_stream_t stream);
+                   int32_t* ids, int sm_count, pnv_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -21,7 +21,7 @@ LINEAR = dict(out=A, out_f32=0, x=A, x_stride=64, w=A, bias=A, bias_f32=0, resid
 MX8 = dict(out=A, x=A, x_sf=A, w=A, w_sf=A, bias=A, bias_f32=0, residual=A, residual_stride=128, rows=5, features=128, k=64, act=2, gated=0,
            beta=1.0, linear_beta=-1.0, sms=0, stream=None)
 ROUTE = dict(logits=A, bf16=0, stride=64, rows=5, experts=64, topk=8, sigmoid=0, bias=A, groups=4, topk_groups=2, renorm=1, scale=1.0, w=A, ids=A,
-             stream=None)
+             sms=0, stream=None)
 
 CASES = [
     ("pnv_add_rms_norm", NORM, [
