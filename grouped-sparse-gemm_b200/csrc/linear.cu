@@ -238,7 +238,9 @@ struct SplitCfg {
   static constexpr int kSumBytes = BN * kTileRows * 4;               // partial sums of this CTA's share of the outputs
   static constexpr int kMaxStages = 12;
   static constexpr int kFit = (kSmemMax - 1024 - kBarBytes - kSumBytes) / kStageBytes;
-  static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
+  // A multiple of the issuers, so that the same one meets every turn of a stage: a wait for a parity cannot tell the turn it wants
+  // from the one two before, so a warp that skips turns may find a stage full that is still being filled.
+  static constexpr int kStages = (kFit < kMaxStages ? kFit : kMaxStages) / kIssuers * kIssuers;
   // stages after which the accumulators are emptied into registers: 512 K in each of the two (float32 results only)
   static constexpr int kChunk = 16;
   // tensor memory: the issuers' accumulators, twice where they are emptied on the way, then the scales
@@ -247,7 +249,7 @@ struct SplitCfg {
   static constexpr int kColsUsed = kColSf + (kMx8 ? 8 * kStages : 0);
   static constexpr int kTmemCols = kColsUsed <= 32 ? 32 : kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kSumBytes + kBarBytes;
-  static_assert(kColsUsed <= 512 && kStages > kIssuers, "tensor-memory column map or pipeline");
+  static_assert(kColsUsed <= 512 && kStages > kIssuers && kStages % kIssuers == 0, "tensor-memory column map or pipeline");
 };
 
 template <int BN, bool kMx8, int kMode>
@@ -319,9 +321,9 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         ptx::mbar_arrive_expect_tx(full + stage, C::kStageBytes);
         ptx::tma_load_3d(st, &map_w, full + stage, ks * kStageRow, ft * kTileRows, 0);
         ptx::tma_load_3d(st + kABytes, &map_x, full + stage, ks * kStageRow, tt * BN, 0);
-        if constexpr (kMx8) {            // (a token tile below 128 is the only one and starts its atom)
+        if constexpr (kMx8) {            // (token tiles of 64 share an atom of scales in twos, narrower ones are the only one)
           ptx::bulk_load(st + kABytes + C::kBBytes, a.w_sf + ((long long)ft * n_kt + ks) * 512, 512, full + stage);
-          ptx::bulk_load(st + kABytes + C::kBBytes + 512, a.x_sf + ((long long)tt * n_kt + ks) * 512, 512, full + stage);
+          ptx::bulk_load(st + kABytes + C::kBBytes + 512, a.x_sf + ((long long)(tt * BN / 128) * n_kt + ks) * 512, 512, full + stage);
         }
       }
       __syncwarp();
@@ -330,6 +332,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   } else if (warp <= kIssuers) {
     // ---- issuers
     const int me = warp - 1;
+    const uint32_t sfb_shift = (uint32_t)(tt * BN & 127) / 32;         // tokens 64 on of an atom: two columns on
     int stage = me;
     uint32_t phase = 0;
     bool ok = true;
@@ -362,7 +365,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             ptx::tc_cp_32x128b_warpx4(sfb, ptx::smem_desc(st + kABytes + C::kBBytes + 512, 128, 0, 0));
           }
           issue_stage<1, kMx8>(d, ptx::smem_desc(st, 1024, 16, 2), ptx::smem_desc(st + kABytes, 1024, 16, 2), product_idesc<kMx8>(BN, kTileRows),
-                               stage_mmas(a.k_bytes, ks0 + i), i == lo, sfa, sfb);
+                               stage_mmas(a.k_bytes, ks0 + i), i == lo, sfa, sfb + sfb_shift);
           ptx::tc_commit(empty + stage);
           if (i + kIssuers >= hi) ptx::tc_commit(acc_full + buf);
         }
@@ -861,40 +864,101 @@ int rows_map(CUtensorMap* map, const void* base, uint64_t width, uint64_t rows, 
   });
 }
 
-constexpr int kFill = 64;                // bytes a CTA takes in from L2 in a cycle
 constexpr int kMaxSplitLog = 3;          // clusters of 1, 2, 4 or 8 CTAs
 
-// Per kernel and device, once: shared-memory carve-out, and how many clusters of each size run at one time.
+// Per kernel and device, once: the shared-memory carve-out.
 struct Setup {
   std::once_flag once[64];
   cudaError_t err[64] = {};
-  int clusters[64][kMaxSplitLog + 1] = {};
 };
-
 template <class Kernel>
-int prepare(Kernel kernel, Setup& s, int threads, size_t smem, const int** clusters) {
+int prepare(Kernel kernel, Setup& s, size_t smem) {
   int dev = 0;
   PNV_CUDA(cudaGetDevice(&dev));
   PNV_REQUIRE(dev >= 0 && dev < 64, "unexpected CUDA device index %d", dev);
-  std::call_once(s.once[dev], [&] {
-    s.err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    for (int i = 0; i <= kMaxSplitLog && s.err[dev] == cudaSuccess; ++i) {
+  std::call_once(s.once[dev], [&] { s.err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
+  if (s.err[dev] != cudaSuccess) return fail(PNV_ERR_CUDA, "linear kernel set-up failed: %s", cudaGetErrorString(s.err[dev]));
+  return PNV_OK;
+}
+
+// Per device, once: how many clusters of 2^i CTAs run at one time.  Every kernel here fills an SM's shared memory with one CTA,
+// so one of them answers for all.
+int cluster_capacity(const int** out) {
+  using C = SplitCfg<16, false>;
+  static Setup setup, asked;
+  static int clusters[64][kMaxSplitLog + 1] = {};
+  const auto kernel = linear_split_kernel<16, false, kNothing>;
+  if (int rc = prepare(kernel, setup, C::kSmem)) return rc;
+  int dev = 0;
+  PNV_CUDA(cudaGetDevice(&dev));
+  std::call_once(asked.once[dev], [&] {
+    for (int i = 0; i <= kMaxSplitLog && asked.err[dev] == cudaSuccess; ++i) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(8 << 7);
-      cfg.blockDim = dim3(threads);
-      cfg.dynamicSmemBytes = smem;
+      cfg.blockDim = dim3(C::kThreads);
+      cfg.dynamicSmemBytes = C::kSmem;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
       attr[0].val.clusterDim.x = 1u << i;
       attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
-      s.err[dev] = cudaOccupancyMaxActiveClusters(&s.clusters[dev][i], kernel, &cfg);
+      asked.err[dev] = cudaOccupancyMaxActiveClusters(&clusters[dev][i], kernel, &cfg);
     }
   });
-  if (s.err[dev] != cudaSuccess) return fail(PNV_ERR_CUDA, "linear kernel set-up failed: %s", cudaGetErrorString(s.err[dev]));
-  *clusters = s.clusters[dev];
+  if (asked.err[dev] != cudaSuccess) return fail(PNV_ERR_CUDA, "linear kernel set-up failed: %s", cudaGetErrorString(asked.err[dev]));
+  *out = clusters[dev];
   return PNV_OK;
+}
+
+// ---- which kernel, tile and split: the cheapest by a model of their time ---------------------------------
+//
+// The constants are a fit, in units of 1/1.9 ns, to measured times of all the candidates for eight weights from 256 x 7168 to
+// 28672 x 4096 and 1 to 4096 tokens, both operand types (two thousand calls): off by a tenth on average; the candidate that it
+// picks is 1.1 % slower than the best one on average and 18 % at worst.
+
+struct Plan {
+  int tokens;                            // split kernel: tokens of a tile; 0: pair kernel
+  int split;                             // split kernel: CTAs that share a tile's K
+  int width;                             // pair kernel: features of a tile
+  long long cost;
+};
+
+Plan make_plan(const LinearArgs& a, bool mx8, const int* clusters, int sm_count) {
+  const long long stages = ceil_div_i(a.k_bytes, kStageRow);
+  Plan best{0, 0, 0, -1};
+  auto offer = [&](const Plan& p) {
+    if (best.cost < 0 || p.cost < best.cost) best = p;
+  };
+  for (int tokens = 16; tokens <= 128; tokens *= 2) {
+    // Tiles no wider than they need be.  (Scale words start at multiples of 64 tokens: narrower tiles only on their own.)
+    if (tokens > 16 && tokens / 2 >= a.rows) break;
+    if (mx8 && tokens < 64 && tokens < a.rows) continue;
+    const long long token_tiles = ceil_div_i(a.rows, tokens), tiles = token_tiles * ceil_div_i(a.features, kTileRows);
+    if (token_tiles > 65535) continue;
+    for (int i = 0; i <= kMaxSplitLog; ++i) {
+      const int split = 1 << i, room = std::min(clusters[i], sm_count >> i);
+      if (room < 1 || (split > 1 && (tiles > room || stages < 2 * split))) continue;
+      const long long waves = (tiles + room - 1) / room, mine = (stages + split - 1) / split;
+      // a stage: what is issued for it, its bytes, or the weights' bytes of all CTAs
+      const long long stage = std::max(std::max(213, 171 + tokens), (int)(std::min<long long>(tiles * split, sm_count) * kABytes / 5670));
+      const long long sums = split > 1 ? 1690 + 20 * tokens + 10 * split : 0;        // on their way between the CTAs
+      offer(Plan{tokens, split, 0, 4360 + waves * (mine * stage + sums + 47 * tokens)});
+    }
+  }
+  const int pairs = std::min(clusters[1], sm_count / 2);
+  if (!a.out_f32 && pairs >= 1) {
+    // Widths of 32 features; of 64 where the scales' atoms or the gates' blocks ask for it.
+    const long long m_tiles = ceil_div_i(a.rows, 256);
+    for (int width = 256; width >= 128; width -= mx8 || a.gated ? 64 : 32) {
+      const long long tiles = m_tiles * ceil_div_i(a.features, width), waves = (tiles + pairs - 1) / pairs;
+      if (tiles >= (1LL << 31) / kBand) continue;
+      // a stage: its products (2 cycles a feature at full clock) and waits; a tile at least what its epilogue takes
+      const long long stage = mx8 ? 236 + 19 * width / 10 : 84 + 23 * width / 10;
+      offer(Plan{0, 1, width, 5760 + waves * std::max(stages * stage, 3980LL) + 10 * width});
+    }
+  }
+  return best;
 }
 
 template <class Kernel, class... Args>
@@ -929,19 +993,10 @@ struct Operands {
 };
 
 template <int BN, bool kMx8, int kMode>
-int split_setup(const int** clusters) {
-  static Setup setup;
-  return prepare(linear_split_kernel<BN, kMx8, kMode>, setup, SplitCfg<BN, kMx8>::kThreads, SplitCfg<BN, kMx8>::kSmem, clusters);
-}
-template <bool kMx8, int kMode>
-int pair_setup(const int** clusters) {
-  static Setup setup;
-  return prepare(linear_pair_kernel<kMx8, kMode>, setup, PairCfg<kMx8>::kThreads, PairCfg<kMx8>::kSmem, clusters);
-}
-
-template <int BN, bool kMx8, int kMode>
 int launch_split(const Operands& o, const LinearArgs& a, int split, cudaStream_t stream) {
   using C = SplitCfg<BN, kMx8>;
+  static Setup setup;
+  if (int rc = prepare(linear_split_kernel<BN, kMx8, kMode>, setup, C::kSmem)) return rc;
   CUtensorMap map_w, map_x;
   if (int rc = operand_map(&map_w, o.w, a.k_bytes, a.features, a.k_bytes, kTileRows)) return rc;
   if (int rc = operand_map(&map_x, o.x, a.k_bytes, a.rows, o.x_stride, BN)) return rc;
@@ -951,8 +1006,14 @@ int launch_split(const Operands& o, const LinearArgs& a, int split, cudaStream_t
 }
 
 template <bool kMx8, int kMode>
-int launch_pair(const Operands& o, LinearArgs a, int pairs, cudaStream_t stream) {
+int launch_pair(const Operands& o, LinearArgs a, int width, int sm_count, cudaStream_t stream) {
   using C = PairCfg<kMx8>;
+  static Setup setup;
+  if (int rc = prepare(linear_pair_kernel<kMx8, kMode>, setup, C::kSmem)) return rc;
+  a.tile_n = width;
+  a.m_tiles = ceil_div_i(a.rows, 256);
+  a.n_tiles = ceil_div_i(a.features, width);
+  const int pairs = std::min(sm_count / 2, a.m_tiles * a.n_tiles);
   CUtensorMap map_w, map_x, map_w_sf = {}, map_x_sf = {}, map_out = {}, map_res = {};
   if (int rc = operand_map(&map_w, o.w, a.k_bytes, a.features, a.k_bytes, a.tile_n / 2)) return rc;
   if (int rc = operand_map(&map_x, o.x, a.k_bytes, a.rows, o.x_stride, 128)) return rc;
@@ -972,48 +1033,18 @@ int launch_pair(const Operands& o, LinearArgs a, int pairs, cudaStream_t stream)
   return PNV_OK;
 }
 
-// Which kernel, and how many CTAs share a tile's K.
 template <bool kMx8, int kMode>
-int run_linear(const Operands& o, LinearArgs a, int sm_count, cudaStream_t stream) {
-  const int k_stages = ceil_div_i(a.k_bytes, kStageRow);
-  const int bn = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : a.rows <= 64 ? 64 : 128;
-  const long long tiles = (long long)ceil_div_i(a.features, kTileRows) * ceil_div_i(a.rows, bn);
+int run_linear(const Operands& o, const LinearArgs& a, int sm_count, cudaStream_t stream) {
   const int* clusters = nullptr;
-  if (int rc = bn == 16 ? split_setup<16, kMx8, kMode>(&clusters) : bn == 32 ? split_setup<32, kMx8, kMode>(&clusters)
-             : bn == 64 ? split_setup<64, kMx8, kMode>(&clusters) : split_setup<128, kMx8, kMode>(&clusters))
-    return rc;
-  int split = 1;
-  for (int i = 1; i <= kMaxSplitLog; ++i)
-    if (tiles <= std::min(clusters[i], sm_count >> i) && (k_stages >> i) >= 2) split = 1 << i;
-  if (!a.out_f32 && bn == 128) {
-    const int* pair_clusters = nullptr;
-    if (int rc = pair_setup<kMx8, kMode>(&pair_clusters)) return rc;
-    const int pairs = std::min(pair_clusters[1], sm_count / 2);
-    const long long m_tiles = ceil_div_i(a.rows, 256);
-    // Cycles of a stage: the products of a pair's tile, 2 per feature, or what a CTA takes in, 64 bytes a cycle, whichever is
-    // more.  (Widths: of 32 features; of 64 where the scales' atoms or the gates' blocks ask for it.)
-    const int step = kMx8 || a.gated ? 64 : 32;
-    long long best = 0;
-    for (int width = 256; pairs >= 1 && width >= 128; width -= step) {
-      const long long tiles_n = ceil_div_i(a.features, width), waves = (m_tiles * tiles_n + pairs - 1) / pairs;
-      const long long cost = waves * std::max(2 * width, (kABytes + width / 2 * kStageRow) / kFill);
-      if (m_tiles * tiles_n < (1LL << 31) / kBand && (best == 0 || cost < best)) {
-        best = cost;
-        a.m_tiles = (int)m_tiles;
-        a.n_tiles = (int)tiles_n;
-        a.tile_n = width;
-      }
-    }
-    const long long split_waves = (tiles * split + sm_count - 1) / sm_count;
-    if (best > 0 && best * split <= split_waves * ((kABytes + 128 * kStageRow) / kFill))
-      return launch_pair<kMx8, kMode>(o, a, (int)std::min<long long>(pairs, m_tiles * a.n_tiles), stream);
-  }
-  PNV_REQUIRE(ceil_div_i(a.rows, bn) <= 65535 && ceil_div_i(a.features, kTileRows) < (1 << 28), "linear: too many rows for one call");
-  switch (bn) {
-    case 16: return launch_split<16, kMx8, kMode>(o, a, split, stream);
-    case 32: return launch_split<32, kMx8, kMode>(o, a, split, stream);
-    case 64: return launch_split<64, kMx8, kMode>(o, a, split, stream);
-    default: return launch_split<128, kMx8, kMode>(o, a, split, stream);
+  if (int rc = cluster_capacity(&clusters)) return rc;
+  const Plan p = make_plan(a, kMx8, clusters, sm_count);
+  PNV_REQUIRE(p.cost >= 0, "linear: too many rows for one call");
+  switch (p.tokens) {
+    case 0: return launch_pair<kMx8, kMode>(o, a, p.width, std::min(2 * clusters[1], sm_count), stream);
+    case 16: return launch_split<16, kMx8, kMode>(o, a, p.split, stream);
+    case 32: return launch_split<32, kMx8, kMode>(o, a, p.split, stream);
+    case 64: return launch_split<64, kMx8, kMode>(o, a, p.split, stream);
+    default: return launch_split<128, kMx8, kMode>(o, a, p.split, stream);
   }
 }
 
