@@ -1121,6 +1121,26 @@ extern "C" int pnv_linear_mx8(void* out, const uint8_t* x, const uint8_t* x_sf, 
                        beta, linear_beta, sm_count, (cudaStream_t)stream);
 }
 
+extern "C" int pnv_linear_plan(int mx8, int64_t rows, int features, int k, int out_is_f32, int gated, int sm_count, int* tokens, int* split,
+                               int* width) {
+  PNV_REQUIRE(tokens && split && width, "null pointer argument");
+  PNV_REQUIRE(rows >= 1 && rows < (1LL << 31) - 256 && features >= 1 && features < (1 << 30) && k >= 1 && k < (1 << 29), "sizes out of range");
+  LinearArgs a{};
+  a.rows = (int)rows;
+  a.features = features;
+  a.k_bytes = mx8 ? k : 2 * k;
+  a.out_f32 = out_is_f32;
+  a.gated = gated;
+  const int* clusters = nullptr;
+  if (int rc = cluster_capacity(&clusters)) return rc;
+  const Plan p = make_plan(a, mx8 != 0, clusters, sm_count > 0 ? sm_count : 148);
+  PNV_REQUIRE(p.cost >= 0, "linear: too many rows for one call");
+  *tokens = p.tokens;
+  *split = p.split;
+  *width = p.width;
+  return PNV_OK;
+}
+
 extern "C" int pnv_linear_device_status(int* status_out) {
   PNV_REQUIRE(status_out, "null pointer argument");
   PNV_CUDA(cudaDeviceSynchronize());

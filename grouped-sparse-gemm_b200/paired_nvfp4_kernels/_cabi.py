@@ -53,6 +53,7 @@ SIGNATURES = {
     "pnv_quant_mx8": (_i, [_p, _i64, _i64, _i, _p, _p, _p]),
     "pnv_linear": (_i, [_p, _i, _p, _i64, _p, _p, _i, _p, _i64, _i64, _i, _i, _i, _i, _f, _f, _i, _p]),
     "pnv_linear_mx8": (_i, [_p, _p, _p, _p, _p, _p, _i, _p, _i64, _i64, _i, _i, _i, _i, _f, _f, _i, _p]),
+    "pnv_linear_plan": (_i, [_i, _i64, _i, _i, _i, _i, _i] + [ctypes.POINTER(_i)] * 3),
     "pnv_linear_device_status": (_i, [ctypes.POINTER(_i)]),
     "pnv_route_topk": (_i, [_p, _i, _i64, _i64, _i, _i, _i, _p, _i, _i, _i, _f, _p, _p, _i, _p]),
     "pnv_peer_buffer_alloc": (_i, [_i64, _p, _p]),

@@ -67,6 +67,15 @@ def group_mm_device_status():
     return v.value
 
 
+def linear_plan(rows, features, k, mx8=False, float_out=False, gated=False):
+    """Which kernel linear or linear_mx8 runs for these sizes on the current device: ("split", tokens of a tile, CTAs that share
+    its K) or ("pair", features of a tile)."""
+    v = [ctypes.c_int() for _ in range(3)]
+    _cabi.check(_lib.pnv_linear_plan(int(mx8), rows, features, k, int(float_out), int(gated), 0, *[ctypes.byref(x) for x in v]))
+    tokens, split, width = (x.value for x in v)
+    return ("split", tokens, split) if tokens else ("pair", width)
+
+
 def linear_device_status():
     """The same for linear and linear_mx8."""
     v = ctypes.c_int()

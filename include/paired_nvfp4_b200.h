@@ -355,6 +355,11 @@ int pnv_linear_mx8(void* out, const uint8_t* x, const uint8_t* x_sf, const uint8
                    int bias_is_f32, const void* residual, int64_t residual_stride, int64_t rows, int features, int k,
                    int act_kind, int gated, float beta, float linear_beta, int sm_count, pnv_stream_t stream);
 
+/* Which kernel a dense layer of these sizes runs on the current device: *tokens > 0: tiles of 128 features x *tokens tokens, the K
+ * of each shared by *split CTAs; *tokens == 0: CTA pairs with tiles of 256 tokens x *width features. */
+int pnv_linear_plan(int mx8, int64_t rows, int features, int k, int out_is_f32, int gated, int sm_count, int* tokens, int* split,
+                    int* width);
+
 /* pnv_group_mm_device_status of the dense kernels. */
 int pnv_linear_device_status(int* status_out);
 
