@@ -925,37 +925,39 @@ struct Plan {
 };
 
 Plan make_plan(const LinearArgs& a, bool mx8, const int* clusters, int sm_count) {
-  const long long stages = ceil_div_i(a.k_bytes, kStageRow);
+  const long long stages = ceil_div_i(a.k_bytes, kStageRow), feature_tiles = ceil_div_i(a.features, kTileRows);
+  const auto waves_of = [](long long tiles, int room) { return tiles <= room ? 1LL : (tiles + room - 1) / room; };
   Plan best{0, 0, 0, -1};
-  auto offer = [&](const Plan& p) {
+  const auto offer = [&](const Plan& p) {
     if (best.cost < 0 || p.cost < best.cost) best = p;
   };
-  for (int tokens = 16; tokens <= 128; tokens *= 2) {
+  for (int log = 4; log <= 7; ++log) {
+    const int tokens = 1 << log;
     // Tiles no wider than they need be.  (Scale words start at multiples of 64 tokens: narrower tiles only on their own.)
     if (tokens > 16 && tokens / 2 >= a.rows) break;
     if (mx8 && tokens < 64 && tokens < a.rows) continue;
-    const long long token_tiles = ceil_div_i(a.rows, tokens), tiles = token_tiles * ceil_div_i(a.features, kTileRows);
-    if (token_tiles > 65535) continue;
+    const long long token_tiles = (a.rows + tokens - 1) >> log, tiles = token_tiles * feature_tiles;
+    if (token_tiles > 65535) continue;   // (a grid's limit)
     for (int i = 0; i <= kMaxSplitLog; ++i) {
       const int split = 1 << i, room = std::min(clusters[i], sm_count >> i);
-      if (room < 1 || (split > 1 && (tiles > room || stages < 2 * split))) continue;
-      const long long waves = (tiles + room - 1) / room, mine = (stages + split - 1) / split;
+      if (room < 1 || (split > 1 && (tiles > room || stages < 2 * split))) break;
+      const long long mine = (stages + split - 1) >> i;
       // a stage: what is issued for it, its bytes, or the weights' bytes of all CTAs
       const long long stage = std::max(std::max(213, 171 + tokens), (int)(std::min<long long>(tiles * split, sm_count) * kABytes / 5670));
       const long long sums = split > 1 ? 1690 + 20 * tokens + 10 * split : 0;        // on their way between the CTAs
-      offer(Plan{tokens, split, 0, 4360 + waves * (mine * stage + sums + 47 * tokens)});
+      offer(Plan{tokens, split, 0, 4360 + waves_of(tiles, room) * (mine * stage + sums + 47 * tokens)});
     }
   }
   const int pairs = std::min(clusters[1], sm_count / 2);
   if (!a.out_f32 && pairs >= 1) {
     // Widths of 32 features; of 64 where the scales' atoms or the gates' blocks ask for it.
-    const long long m_tiles = ceil_div_i(a.rows, 256);
+    const long long m_tiles = (a.rows + 255) >> 8;
     for (int width = 256; width >= 128; width -= mx8 || a.gated ? 64 : 32) {
-      const long long tiles = m_tiles * ceil_div_i(a.features, width), waves = (tiles + pairs - 1) / pairs;
+      const long long tiles = m_tiles * ((a.features + width - 1) / width);
       if (tiles >= (1LL << 31) / kBand) continue;
       // a stage: its products (2 cycles a feature at full clock) and waits; a tile at least what its epilogue takes
       const long long stage = mx8 ? 236 + 19 * width / 10 : 84 + 23 * width / 10;
-      offer(Plan{0, 1, width, 5760 + waves * std::max(stages * stage, 3980LL) + 10 * width});
+      offer(Plan{0, 1, width, 5760 + waves_of(tiles, pairs) * std::max(stages * stage, 3980LL) + 10 * width});
     }
   }
   return best;

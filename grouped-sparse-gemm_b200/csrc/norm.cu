@@ -123,10 +123,14 @@ add_rms_norm_kernel(const NormArgs a) {
       for (int p = 0; p < V; ++p) unpack8(raw[p], v[p]);
     }
   }
+  // squares are added eight by eight, then those sums: in one chain of 40 the roundings add up to what moves a code in a million
 #pragma unroll
-  for (int p = 0; p < V; ++p)
+  for (int p = 0; p < V; ++p) {
+    float s[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum = fmaf(v[p][j], v[p][j], sum);
+    for (int j = 0; j < 4; ++j) s[j] = fmaf(v[p][2 * j + 1], v[p][2 * j + 1], v[p][2 * j] * v[p][2 * j]);
+    sum += (s[0] + s[1]) + (s[2] + s[3]);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (a.team > 32) {
