@@ -632,7 +632,39 @@ group_mm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 
 // ---- host side -----------------------------------------------------------------------------------
 
+// Tensor maps are pure functions of (base pointer, extents, box, swizzle).  A serving loop calls with
+// the same few operand buffers over and over, so the most recent maps are kept and the driver's
+// encoder is only called for a new key.  A map holds no reference to the memory it describes: a
+// buffer freed and reallocated at the same address with the same shape yields the same map.
+struct MapKey {
+  const void* base;
+  uint64_t row_bytes, rows, experts;
+  uint32_t box_rows, box_inner, kind;   // kind: 0 = 3-D tile, 1 = 4-D activation view; swizzle in the high bits
+  bool operator==(const MapKey& o) const {
+    return base == o.base && row_bytes == o.row_bytes && rows == o.rows && experts == o.experts &&
+           box_rows == o.box_rows && box_inner == o.box_inner && kind == o.kind;
+  }
+};
+constexpr int kMapCacheSize = 64;
+struct MapCache {
+  std::mutex mu;
+  MapKey keys[kMapCacheSize];
+  CUtensorMap maps[kMapCacheSize];
+  int used = 0, next = 0;
+};
 MapCache g_maps;
+
+template <class Encode>
+int cached_map(CUtensorMap* out, const MapKey& key, Encode encode) {
+  std::lock_guard<std::mutex> lock(g_maps.mu);
+  for (int i = 0; i < g_maps.used; ++i)
+    if (g_maps.keys[i] == key) { *out = g_maps.maps[i]; return PNV_OK; }
+  if (int rc = encode(out)) return rc;
+  const int slot = g_maps.used < kMapCacheSize ? g_maps.used++ : (g_maps.next++ % kMapCacheSize);
+  g_maps.keys[slot] = key;
+  g_maps.maps[slot] = *out;
+  return PNV_OK;
+}
 
 // 4-D view of the activations [experts][K/256 chunks][rows][128 B] for K a multiple of 256: one box
 // [chunks][box_rows][128 B] is `chunks` consecutive 128-byte-swizzled operand tiles in shared memory.
@@ -640,7 +672,7 @@ int make_map_b4(CUtensorMap* map, const void* base, uint64_t row_bytes, uint64_t
                 uint32_t box_rows, uint32_t box_chunks) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-  return cached_map(g_maps, map, MapKey{base, row_bytes, rows, experts, box_rows, box_chunks, 1u}, [&](CUtensorMap* m) {
+  return cached_map(map, MapKey{base, row_bytes, rows, experts, box_rows, box_chunks, 1u}, [&](CUtensorMap* m) {
     cuuint64_t dims[4] = {128, rows, row_bytes / 128, experts};
     cuuint64_t strides[3] = {row_bytes, 128, row_bytes * rows};
     cuuint32_t box[4] = {128, box_rows, box_chunks, 1};
@@ -660,7 +692,7 @@ int make_map(CUtensorMap* map, const void* base, uint64_t row_bytes, uint64_t ro
              uint32_t box_bytes, uint32_t box_rows, CUtensorMapSwizzle swz) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-  return cached_map(g_maps, map, MapKey{base, row_bytes, rows, experts, box_rows, box_bytes, (uint32_t)swz << 8}, [&](CUtensorMap* m) {
+  return cached_map(map, MapKey{base, row_bytes, rows, experts, box_rows, box_bytes, (uint32_t)swz << 8}, [&](CUtensorMap* m) {
     cuuint64_t dims[3] = {row_bytes, rows, experts};
     cuuint64_t strides[2] = {row_bytes, row_bytes * rows};
     cuuint32_t box[3] = {box_bytes, box_rows, 1};
@@ -679,7 +711,7 @@ int make_map(CUtensorMap* map, const void* base, uint64_t row_bytes, uint64_t ro
 int make_map_out(CUtensorMap* map, const void* base, uint64_t features, uint64_t rows, uint64_t experts, uint32_t box_rows) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-  return cached_map(g_maps, map, MapKey{base, features * 2, rows, experts, box_rows, 64, 2u}, [&](CUtensorMap* m) {
+  return cached_map(map, MapKey{base, features * 2, rows, experts, box_rows, 64, 2u}, [&](CUtensorMap* m) {
     cuuint64_t dims[3] = {features, rows, experts};
     cuuint64_t strides[2] = {features * 2, features * 2 * rows};
     cuuint32_t box[3] = {64, box_rows, 1};

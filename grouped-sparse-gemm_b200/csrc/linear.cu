@@ -807,61 +807,39 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 
 // ---- host side -------------------------------------------------------------------------------------
 
-MapCache g_linear_maps;
-
-// An operand [rows][k_bytes], rows `stride` bytes apart, in boxes of box_rows x 128 bytes (128-byte swizzle).
-int operand_map(CUtensorMap* map, const void* base, uint64_t k_bytes, uint64_t rows, uint64_t stride, uint32_t box_rows) {
+// A tiled view [rows][width] of `type`, rows `stride` bytes apart, in boxes of box_rows x box_width.  (Encoding one takes a
+// third of a microsecond.)
+int make_view(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t width, uint64_t rows, uint64_t stride, uint32_t box_width,
+              uint32_t box_rows, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion, uint64_t layers = 1, uint32_t box_layers = 1) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-  return cached_map(g_linear_maps, map, MapKey{base, k_bytes, rows, stride, box_rows, kStageRow, 0u}, [&](CUtensorMap* m) {
-    cuuint64_t dims[3] = {k_bytes, rows, 1};
-    cuuint64_t strides[2] = {stride, stride * rows};
-    cuuint32_t box[3] = {kStageRow, box_rows, 1};
-    cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS)
-      return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled (operand) failed with CUresult %d (row_bytes=%llu rows=%llu)", (int)r,
-                  (unsigned long long)k_bytes, (unsigned long long)rows);
-    return (int)PNV_OK;
-  });
+  cuuint64_t dims[3] = {width, rows, layers};
+  cuuint64_t strides[2] = {stride, stride * rows};
+  cuuint32_t box[3] = {box_width, box_rows, box_layers};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, type, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (width=%llu rows=%llu stride=%llu)", (int)r,
+                (unsigned long long)width, (unsigned long long)rows, (unsigned long long)stride);
+  return PNV_OK;
 }
 
+// An operand [rows][k_bytes] in boxes of 128 bytes of K (128-byte swizzle).
+int operand_map(CUtensorMap* map, const void* base, uint64_t k_bytes, uint64_t rows, uint64_t stride, uint32_t box_rows) {
+  return make_view(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, k_bytes, rows, stride, kStageRow, box_rows, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
 // A scale buffer as [row atoms][K atoms][128 words], in boxes of `atoms` row atoms of one K atom.  (A tiled copy, unlike a
 // plain bulk copy, can count its bytes on the partner's barrier.)
 int scale_map(CUtensorMap* map, const void* base, uint64_t row_atoms, uint64_t k_atoms, uint32_t atoms) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-  return cached_map(g_linear_maps, map, MapKey{base, k_atoms, row_atoms, 0, atoms, 128, 1u}, [&](CUtensorMap* m) {
-    cuuint64_t dims[3] = {128, k_atoms, row_atoms};
-    cuuint64_t strides[2] = {512, 512 * k_atoms};
-    cuuint32_t box[3] = {128, 1, atoms};
-    cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS)
-      return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled (scales) failed with CUresult %d (row atoms=%llu, K atoms=%llu)", (int)r,
-                  (unsigned long long)row_atoms, (unsigned long long)k_atoms);
-    return (int)PNV_OK;
-  });
+  return make_view(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 128, k_atoms, 512, 128, 1, CU_TENSOR_MAP_SWIZZLE_NONE,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, row_atoms, atoms);
 }
-
-// bf16 rows [rows][width], `stride` elements apart, in boxes of 32 x 32 (64-byte swizzle): outputs and residuals.
+// bf16 rows, `stride` elements apart, in boxes of 32 x 32 (64-byte swizzle): outputs and residuals.
 int rows_map(CUtensorMap* map, const void* base, uint64_t width, uint64_t rows, uint64_t stride) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-  return cached_map(g_linear_maps, map, MapKey{base, width, rows, stride, 32, 32, 2u}, [&](CUtensorMap* m) {
-    cuuint64_t dims[3] = {width, rows, 1};
-    cuuint64_t strides[2] = {stride * 2, stride * 2 * rows};
-    cuuint32_t box[3] = {32, 32, 1};
-    cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS)
-      return fail(PNV_ERR_CUDA, "cuTensorMapEncodeTiled (rows) failed with CUresult %d (width=%llu rows=%llu)", (int)r,
-                  (unsigned long long)width, (unsigned long long)rows);
-    return (int)PNV_OK;
-  });
+  return make_view(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, width, rows, stride * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_NONE);
 }
 
 constexpr int kMaxSplitLog = 3;          // clusters of 1, 2, 4 or 8 CTAs
