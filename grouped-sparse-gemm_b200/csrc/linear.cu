@@ -8,8 +8,17 @@
 //            as a decode step wants.  Where there are fewer tiles than SMs a cluster of up to eight CTAs shares a tile's K and
 //            sends its partial sums to the CTAs that own their tokens by copies between their shared memories, which add them in a
 //            fixed order: no workspace, no atomics.
-//   pair     persistent; a CTA pair multiplies 256 tokens x 256 weight rows with one instruction, tokens along M, so that a
-//            thread of the epilogue holds neighbouring features of one token.  Large products.
+//   pair     persistent; a CTA pair multiplies 256 tokens x 128 to 256 weight rows with one instruction, tokens along M, so that
+//            a thread of the epilogue holds neighbouring features of one token.  Large products.
+//
+// What bounds them, and measured times (an idle part's clock; a library product of the same operands, without bias, activation
+// and residual, in parentheses):
+//   pair     the tensor pipe, and above a few hundred microseconds the power limit: 8192 x 28672 x 4096 gated 1150 us, 1.67
+//            PFLOP/s, tensor pipe 89 % busy (1190); the same in a loop of seconds 1386 us (1390).  8-bit operands: 8192 x 7168 x
+//            2048 91 us (84), with a residual 104; in a loop 108 and 124 (103).
+//   split    latency where little is read: 16 x 256 x 7168 to float32 4.7 us (10.7); what a CTA takes in, 85 bytes a cycle, and
+//            the way of the partial sums, 16 bytes a cycle, otherwise: 64 x 4096 x 7168 gated on 8-bit operands 8.4 us, 30 MB
+//            (12.9).
 //
 // Accumulation.  The tensor core adds to its fp32 accumulators with truncation: over K = 7168 the sums of random products
 // come out 7e-6 too small in magnitude (relative 8e-6, against 3e-7 of fp32 arithmetic).  That is nothing beside a rounding
@@ -495,6 +504,11 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 }
 
 // ---- pair kernel -----------------------------------------------------------------------------------
+//
+// Six stages of 32 KB (8-bit operands: five of 34 KB with the scales) beside 32 KB in which residuals arrive and outputs leave:
+// with twice that for the epilogue and a stage less the products waited (8192 x 7168 x 2048: 83 us instead of 77).  Eight
+// epilogue warps: a thread keeps its 128 accumulators in registers, so that the one accumulator of 8-bit operands (the scale
+// words need the other's columns) is free again after 130 cycles.
 
 template <bool kMx8>
 struct PairCfg {

@@ -172,7 +172,8 @@ add_rms_norm_kernel(const NormArgs a) {
 constexpr int kQuantThreads = 256;
 
 // A lane takes a block of 32 elements, four lanes the blocks of one word of scales ("quad": 128 elements of a row).  Quads
-// of all rows are laid end to end, rows padded to whole atoms among them: their scales are written here too.
+// of all rows are laid end to end, rows padded to whole atoms among them: their scales are written here too.  Bound: HBM
+// (8192 x 14336: 53 us, 356 MB at 6.7 TB/s).
 __global__ void __launch_bounds__(kQuantThreads)
 quant_mx8_kernel(const __nv_bfloat16* __restrict__ x, long long x_stride, unsigned rows, unsigned quads, int K, int n_kt,
                  uint8_t* __restrict__ q, uint8_t* __restrict__ q_sf) {

