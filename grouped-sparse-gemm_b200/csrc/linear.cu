@@ -1085,7 +1085,7 @@ int linear_common(bool mx8, void* out, int out_is_f32, const void* x, long long 
   a.gated = gated;
   a.kind = act_kind;
   // (pieces of a row start at multiples of 8 outputs)
-  a.vec_out = n_out * (out_is_f32 ? 4 : 2) % 16 == 0 && at(out, 16);
+  a.vec_out = (long long)n_out * (out_is_f32 ? 4 : 2) % 16 == 0 && at(out, 16);
   a.vec_residual = residual_stride % 8 == 0 && at(residual, 16);
   a.vec_bias = at(bias, 16);
   if (sm_count <= 0) sm_count = 148;

@@ -653,7 +653,7 @@ int check_bias(const optional<Tensor>& bias, const Tensor& like, int64_t n, cons
   return is_float(*bias) ? 1 : 0;
 }
 
-// (y, residual_out, q, q_sf); what was not asked for is empty
+// (y, residual_out, q, q_sf); None for what was not asked for
 std::tuple<Tensor, Tensor, Tensor, Tensor> add_rms_norm(const Tensor& x, const optional<Tensor>& residual, const Tensor& weight, double eps,
                                                         bool out_bf16, bool out_mx8) {
   TORCH_CHECK(x.is_cuda() && weight.is_cuda(), "inputs must be CUDA tensors");
@@ -670,10 +670,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> add_rms_norm(const Tensor& x, const o
     check_rows(*residual, "residual must be bf16 [T, hidden] with contiguous rows");
     TORCH_CHECK(residual->size(0) == T && residual->size(1) == H, "residual must be shaped like x");
   }
-  Tensor y = empty_on(x, {out_bf16 ? T : 0, H}, at::kBFloat16);
-  Tensor r = empty_on(x, {residual.has_value() ? T : 0, H}, at::kBFloat16);
-  Tensor q = empty_on(x, {out_mx8 ? T : 0, H}, at::kFloat8_e4m3fn);
-  Tensor q_sf = empty_on(x, {out_mx8 ? pnv_sf_numel((int)T, (int)H, 1) : 0}, at::kFloat8_e8m0fnu);
+  Tensor y, r, q, q_sf;
+  if (out_bf16) y = empty_on(x, {T, H}, at::kBFloat16);
+  if (residual.has_value()) r = empty_on(x, {T, H}, at::kBFloat16);
+  if (out_mx8) {
+    q = empty_on(x, {T, H}, at::kFloat8_e4m3fn);
+    q_sf = empty_on(x, {pnv_sf_numel((int)T, (int)H, 1)}, at::kFloat8_e8m0fnu);
+  }
   if (T == 0) return {y, r, q, q_sf};
   const c10::cuda::CUDAGuard guard(x.device());
   check_rc(pnv_add_rms_norm(x.const_data_ptr(), row_stride(x), residual.has_value() ? residual->const_data_ptr() : nullptr,

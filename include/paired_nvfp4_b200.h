@@ -344,7 +344,8 @@ int pnv_quant_mx8(const void* x, int64_t x_stride, int64_t rows, int k, uint8_t*
  * NULL; residual bf16, rows residual_stride apart, or NULL; out bf16 or float32, contiguous.  act_kind: PNV_ACT_NONE, _RELU,
  * _SILU, _GELU (with erf).  gated: act_kind PNV_ACT_SILU or _SITU, the rows of w (and bias) are gates and ups in 64-row blocks
  * (32 gates, their 32 ups; features a multiple of 64), out[rows, features / 2] = act(gate) * up + residual.
- * float32 outputs are good to 1e-6 of the sum's scale (partial sums are carried out of the tensor core every 512 K). */
+ * float32 outputs are good to 1e-6 of the sum's scale (partial sums are carried out of the tensor core every 512 K) and take at
+ * most 65535 tiles of 128 rows. */
 int pnv_linear(void* out, int out_is_f32, const void* x, int64_t x_stride, const void* w, const void* bias, int bias_is_f32,
                const void* residual, int64_t residual_stride, int64_t rows, int features, int k, int act_kind, int gated,
                float beta, float linear_beta, int sm_count, pnv_stream_t stream);
@@ -366,8 +367,8 @@ int pnv_linear_device_status(int* status_out);
 /* Router logits (float32 or bf16, rows `stride` apart) to expert ids int32[rows, topk], best first, and their weights
  * float32[rows, topk].  Scores: softmax over the experts, or sigmoid.  Experts are ranked by score + bias (float32[experts]),
  * by the logit where bias is NULL; of several groups of neighbouring experts only the topk_groups best take part, ranked by the
- * sum of their two best keys (their best without a bias).  Ties go to the lower index, NaN ranks last.  Keys that 32 bits cannot
- * order are compared in 64.  weights = scores of the chosen (without the bias), divided by their sum if renormalize, times
+ * sum of their two best keys (their best without a bias).  Ties go to the lower index, NaN ranks last (softmax scores are all NaN in a row that has
+ * one: with a bias, or not renormalized).  Keys that 32 bits cannot order are compared in 64.  weights = scores of the chosen (without the bias), divided by their sum if renormalize, times
  * scale; a row of nothing but -infinity has weights 0 with softmax, one whose chosen scores add up to 0 when renormalized. */
 #define PNV_ROUTE_MAX_EXPERTS 1024
 int pnv_route_topk(const void* logits, int logits_are_bf16, int64_t stride, int64_t rows, int experts, int topk, int sigmoid,

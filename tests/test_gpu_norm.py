@@ -55,14 +55,14 @@ def test_norm_matches_64_bits(ops, rows, width, residual, weight_type):
     if residual:
         assert torch.equal(res.cpu(), (x.cpu().float() + r.cpu().float()).to(torch.bfloat16))
     else:
-        assert res.shape == (0, width)
+        assert res is None
     if mx8:
         check_codes(q, sf, n, rows, width)
         only, _, q2, sf2 = ops.add_rms_norm(x, r, w, 1e-6, False, True)
-        assert only.shape == (0, width) and torch.equal(q2.view(torch.uint8), q.view(torch.uint8))
+        assert only is None and torch.equal(q2.view(torch.uint8), q.view(torch.uint8))
         assert torch.equal(sf2.view(torch.uint8), sf.view(torch.uint8))
     else:
-        assert q.numel() == 0 and sf.numel() == 0
+        assert q is None and sf is None
 
 
 # slices of wider rows at element offsets that 16-byte accesses cannot take, and at ones they can
@@ -79,8 +79,8 @@ def test_strided_rows(ops, rows, width, pad, offset):
 
 def test_weight_at_an_odd_element(ops):
     x, w = make(4, 256, 7), make(1, 257, 8)[0]
-    got = ops.add_rms_norm(x, None, w[1:], 1e-6, True, True)
-    want = ops.add_rms_norm(x, None, w[1:].clone(), 1e-6, True, True)
+    got = ops.add_rms_norm(x, x, w[1:], 1e-6, True, True)
+    want = ops.add_rms_norm(x, x, w[1:].clone(), 1e-6, True, True)
     for a, b in zip(got, want):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
