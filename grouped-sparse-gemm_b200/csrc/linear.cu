@@ -14,7 +14,7 @@
 // What bounds them, and measured times (an idle part's clock; a library product of the same operands, without bias, activation
 // and residual, in parentheses):
 //   pair     the tensor pipe, and above a few hundred microseconds the power limit: 8192 x 28672 x 4096 gated 1150 us, 1.67
-//            PFLOP/s, tensor pipe 89 % busy (1190); the same in a loop of seconds 1386 us (1390).  8-bit operands: 8192 x 7168 x
+//            PFLOP/s, tensor pipe 89 % busy (1190); the same in a loop of seconds 1350 us (1390).  8-bit operands: 8192 x 7168 x
 //            2048 91 us (84), with a residual 104; in a loop 108 and 124 (103).
 //   split    latency where little is read: 16 x 256 x 7168 to float32 4.7 us (10.7); what a CTA takes in, 85 bytes a cycle, and
 //            the way of the partial sums, 16 bytes a cycle, otherwise: 64 x 4096 x 7168 gated on 8-bit operands 8.4 us, 30 MB
@@ -57,7 +57,7 @@ struct LinearArgs {
   long long residual_stride;
   int rows, features, n_out;             // n_out: features, or half of them (gated)
   int k_bytes;                           // bytes of K in a row of either operand
-  int m_tiles, n_tiles, tile_n;          // pair kernel: along tokens and along features, and the features of a tile
+  int m_tiles, n_tiles, tile_n, band;    // pair kernel: along tokens and along features, the features of a tile, tiles of a band
   int out_f32, bias_f32, gated, kind;    // kind: PNV_ACT_*
   GatedAct act;
   int vec_out, vec_residual, vec_bias;   // may these be accessed 16 bytes at a time
@@ -529,19 +529,23 @@ struct PairCfg {
   static_assert(kColSf + (kMx8 ? 12 * kStages : 0) <= kTmemCols, "tensor-memory column map overflows");
 };
 
-// Tiles in bands of eight along the tokens (2048 of them), features outer within a band: the tiles that run at one time share
-// activations and weights in L2.
-constexpr int kBand = 8;
-__device__ __forceinline__ void pair_tile(int tile, int m_tiles, int n_tiles, int& mt, int& nt) {
-  const int band = tile / (kBand * n_tiles), in = tile - band * kBand * n_tiles;
-  const int height = min(kBand, m_tiles - band * kBand);
+// Tiles in bands along the tokens, features outer within a band: the tiles that run at one time share activations and weights
+// in L2, and the weights are read from memory once per band.
+__device__ __forceinline__ void pair_tile(int tile, const LinearArgs& a, int& mt, int& nt) {
+  const int band = tile / (a.band * a.n_tiles), in = tile - band * a.band * a.n_tiles;
+  const int height = min(a.band, a.m_tiles - band * a.band);
   nt = in / height;
-  mt = band * kBand + in - nt * height;
+  mt = band * a.band + in - nt * height;
 }
+// Eight tiles of 256 tokens, or 16 or 32 where their activations fill no more than a third of L2.  In loops of seconds, 8192 x
+// 28672 x 4096: 8 / 16 / 32 tiles take 1385 / 1350 / 1467 us, 8-bit operands 780 / 752 / 745; 16384 x 4096 x 14336 1501 / 1560 /
+// 1655.
+constexpr int kLowBand = 8, kHighBand = 32;
+constexpr long long kBandBytes = 40LL << 20;
 
 __device__ __forceinline__ int tile_nt(int tile, const LinearArgs& a) {
   int mt, nt;
-  pair_tile(tile, a.m_tiles, a.n_tiles, mt, nt);
+  pair_tile(tile, a, mt, nt);
   return nt;
 }
 
@@ -599,7 +603,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll 1
     for (int tile = (int)blockIdx.x / 2; ok && tile < tiles; tile += pairs) {
       int mt, nt;
-      pair_tile(tile, a.m_tiles, a.n_tiles, mt, nt);
+      pair_tile(tile, a, mt, nt);
 #pragma unroll 1
       for (int ks = 0; ks < k_stages; ++ks) {
         if (!ptx::mbar_wait_warp(empty + stage, phase ^ 1)) {
@@ -685,14 +689,14 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const int last_blocks = (a.tile_n + 63) / 64;
     if (staged_res && group < last_blocks && (int)blockIdx.x / 2 < tiles && lane == 0) {
       int mt, nt;
-      pair_tile((int)blockIdx.x / 2, a.m_tiles, a.n_tiles, mt, nt);
+      pair_tile((int)blockIdx.x / 2, a, mt, nt);
       ask(mt * 256 + (int)rank * 128 + quarter * 32, nt, group);
     }
     __syncwarp();
 #pragma unroll 1
     for (int tile = (int)blockIdx.x / 2; ok && tile < tiles; tile += pairs) {
       int mt, nt;
-      pair_tile(tile, a.m_tiles, a.n_tiles, mt, nt);
+      pair_tile(tile, a, mt, nt);
       const int row0 = mt * 256 + (int)rank * 128 + quarter * 32, row = row0 + lane;
       float bias[2][2];
 #pragma unroll
@@ -800,7 +804,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
               ask(row0, nt, block + 2);
             } else if (tile + pairs < tiles) {
               int mt2, nt2;
-              pair_tile(tile + pairs, a.m_tiles, a.n_tiles, mt2, nt2);
+              pair_tile(tile + pairs, a, mt2, nt2);
               ask(mt2 * 256 + (int)rank * 128 + quarter * 32, nt2, group);
             }
           }
@@ -946,7 +950,7 @@ Plan make_plan(const LinearArgs& a, bool mx8, const int* clusters, int sm_count)
     const long long m_tiles = (a.rows + 255) >> 8;
     for (int width = 256; width >= 128; width -= mx8 || a.gated ? 64 : 32) {
       const long long tiles = m_tiles * ((a.features + width - 1) / width);
-      if (tiles >= (1LL << 31) / kBand) continue;
+      if (tiles >= (1LL << 31) / kHighBand) continue;
       // a stage: its products (2 cycles a feature at full clock) and waits; a tile at least what its epilogue takes
       const long long stage = mx8 ? 236 + 19 * width / 10 : 84 + 23 * width / 10;
       offer(Plan{0, 1, width, 5760 + waves_of(tiles, pairs) * std::max(stages * stage, 3980LL) + 10 * width});
@@ -1007,6 +1011,8 @@ int launch_pair(const Operands& o, LinearArgs a, int width, int sm_count, cudaSt
   a.tile_n = width;
   a.m_tiles = ceil_div_i(a.rows, 256);
   a.n_tiles = ceil_div_i(a.features, width);
+  a.band = kLowBand;
+  while (a.band < kHighBand && 2LL * a.band * 256 * a.k_bytes <= kBandBytes) a.band *= 2;
   const int pairs = std::min(sm_count / 2, a.m_tiles * a.n_tiles);
   CUtensorMap map_w, map_x, map_w_sf = {}, map_x_sf = {}, map_out = {}, map_res = {};
   if (int rc = operand_map(&map_w, o.w, a.k_bytes, a.features, a.k_bytes, a.tile_n / 2)) return rc;
