@@ -46,7 +46,7 @@ def build(force=False, ptxas_v=False, verbose=True):
     if force or not up_to_date(OUT, _inputs()):
         nvcc = os.environ.get("NVCC", os.path.join(_cuda_home(), "bin", "nvcc"))
         cmd = [nvcc, "-shared", "-Xcompiler", "-fPIC", "-std=c++17", "-O3", "-lineinfo",
-               "-gencode", "arch=compute_100a,code=sm_100a", "-o", OUT]
+               "--threads", "0", "-gencode", "arch=compute_100a,code=sm_100a", "-o", OUT]      # (files side by side)
         if ptxas_v or os.environ.get("PAIRED_NVFP4_PTXAS_V") == "1":
             cmd += ["-Xptxas", "-v"]
         cmd += os.environ.get("PAIRED_NVFP4_NVCC_FLAGS", "").split()      # developer builds, e.g. -DPNV_WIDE_PROFILE

@@ -31,50 +31,88 @@ struct NormArgs {
   float eps;
 };
 
-// Eight neighbouring elements; kVec: as one 16-byte load, else one by one and zeros from `width` on.
-template <bool kVec>
-__device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int i, int width) {
-  if constexpr (kVec) {
-    return __ldg(reinterpret_cast<const uint4*>(row) + i);
+// How a lane reaches the eight neighbouring elements of one of its pieces, piece i of a row.
+//   kWhole    elements 8 i to 8 i + 7, one 16-byte access
+//   kShifted  rows that start anywhere, at the same place within 16 bytes in every buffer: elements 8 i - s on, where s is how far
+//             the row starts behind a 16-byte boundary, so that all accesses but a row's first and last are whole
+//   kSingle   elements 8 i on, one by one
+enum Access : int { kWhole = 0, kShifted = 1, kSingle = 2 };
+
+// Elements at, at + 1, ... of a row of `width` (zeros outside of it).
+template <int kAccess>
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int at, int width) {
+  if constexpr (kAccess == kWhole) {
+    return __ldg(reinterpret_cast<const uint4*>(row + at));
   } else {
+    if (kAccess == kShifted && at >= 0 && at + 8 <= width) return __ldg(reinterpret_cast<const uint4*>(row + at));
     uint32_t h[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      h[j] = i * 8 + j < width ? __ldg(reinterpret_cast<const unsigned short*>(row) + i * 8 + j) : 0u;
+      h[j] = at + j >= 0 && at + j < width ? __ldg(reinterpret_cast<const unsigned short*>(row) + at + j) : 0u;
     return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
   }
 }
-template <bool kVec>
-__device__ __forceinline__ void store8(__nv_bfloat16* row, int i, int width, const float (&f)[8]) {
+template <int kAccess>
+__device__ __forceinline__ void store8(__nv_bfloat16* row, int at, int width, const float (&f)[8]) {
   uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) w[j] = as_u32(__floats2bfloat162_rn(f[2 * j], f[2 * j + 1]));
-  if constexpr (kVec) {
-    reinterpret_cast<uint4*>(row)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  if (kAccess == kWhole || (kAccess == kShifted && at >= 0 && at + 8 <= width)) {
+    *reinterpret_cast<uint4*>(row + at) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (i * 8 + j < width)
-        reinterpret_cast<unsigned short*>(row)[i * 8 + j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
+      if (at + j >= 0 && at + j < width)
+        reinterpret_cast<unsigned short*>(row)[at + j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
   }
 }
-template <bool kVec>
-__device__ __forceinline__ void load_weight8(const void* weight, int f32, int i, int width, float (&w)[8]) {
-  if (!f32) {
-    unpack8(load8<kVec>(static_cast<const __nv_bfloat16*>(weight), i, width), w);
-  } else if (kVec) {
-    const float4 a = __ldg(static_cast<const float4*>(weight) + 2 * i), b = __ldg(static_cast<const float4*>(weight) + 2 * i + 1);
-    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
-  } else {
+// Eight weights from element `at` on.  Shifted, they are cut out of the two whole pieces that hold them: shift = elements by which
+// `at` is short of the second one's start, the same for a row.
+template <int kAccess>
+__device__ __forceinline__ void load_weight8(const void* weight, int f32, int at, int shift, int width, float (&w)[8]) {
+  if (f32) {
+    const float* p = static_cast<const float*>(weight) + at;
+    if (kAccess == kWhole) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+      w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = i * 8 + j < width ? __ldg(static_cast<const float*>(weight) + i * 8 + j) : 0.f;
+      for (int j = 0; j < 8; ++j) w[j] = at + j >= 0 && at + j < width ? __ldg(p + j) : 0.f;
+    }
+    return;
+  }
+  const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(weight);
+  if constexpr (kAccess != kShifted) {
+    unpack8(load8<kAccess>(p, at, width), w);
+  } else {
+    const uint4 hi = load8<kShifted>(p, at + shift, width);
+    if (shift == 0) {
+      unpack8(hi, w);
+      return;
+    }
+    const uint4 lo = load8<kShifted>(p, at + shift - 8, width);
+    uint32_t v[9] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w, 0u};
+    const int skip = 8 - shift;          // elements of the first piece that are not wanted
+    if (skip & 4) {
+#pragma unroll
+      for (int j = 0; j < 6; ++j) v[j] = v[j + 2];
+    }
+    if (skip & 2) {
+#pragma unroll
+      for (int j = 0; j < 5; ++j) v[j] = v[j + 1];
+    }
+    if (skip & 1) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = __funnelshift_r(v[j], v[j + 1], 16);
+    }
+    unpack8(make_uint4(v[0], v[1], v[2], v[3]), w);
   }
 }
 
 // A team of `team` threads takes a row and keeps all of it in registers, V pieces of eight elements a thread, so that
 // memory is read once.  Bound: HBM (9 bytes and 1/32 per element with both outputs): 16384 x 7168 at 6.36 TB/s, 0.97 of a copy.
-template <int V, bool kVec>
+template <int V, int kAccess>
 __global__ void __launch_bounds__(512)
 add_rms_norm_kernel(const NormArgs a) {
   __shared__ float s_sum[16];
@@ -89,7 +127,8 @@ add_rms_norm_kernel(const NormArgs a) {
       for (int i = lane; i < n_kt; i += a.team) *reinterpret_cast<uint32_t*>(sf_row + i * 512LL) = kMx8SlopWord;
     return;
   }
-  const int n = (a.width + kVecElems - 1) / kVecElems;
+  const int shift = kAccess == kShifted ? (int)((unsigned)row * (unsigned)a.width & 7u) : 0;
+  const int n = (a.width + shift + kVecElems - 1) / kVecElems;
   const __nv_bfloat16* x = a.x + row * a.x_stride;
   float v[V][8];
   float sum = 0.f;
@@ -98,7 +137,7 @@ add_rms_norm_kernel(const NormArgs a) {
 #pragma unroll
     for (int p = 0; p < V; ++p) {
       const int i = p * a.team + lane;
-      raw[p] = i < n ? load8<kVec>(x, i, a.width) : make_uint4(0u, 0u, 0u, 0u);
+      raw[p] = i < n ? load8<kAccess>(x, 8 * i - shift, a.width) : make_uint4(0u, 0u, 0u, 0u);
     }
     if (a.residual != nullptr) {
       const __nv_bfloat16* r = a.residual + row * a.residual_stride;
@@ -106,7 +145,7 @@ add_rms_norm_kernel(const NormArgs a) {
 #pragma unroll
       for (int p = 0; p < V; ++p) {
         const int i = p * a.team + lane;
-        more[p] = i < n ? load8<kVec>(r, i, a.width) : make_uint4(0u, 0u, 0u, 0u);
+        more[p] = i < n ? load8<kAccess>(r, 8 * i - shift, a.width) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
       for (int p = 0; p < V; ++p) {
@@ -116,7 +155,7 @@ add_rms_norm_kernel(const NormArgs a) {
         unpack8(more[p], f);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[p][j] += f[j];
-        if (i < n) store8<kVec>(a.residual_out + row * a.width, i, a.width, v[p]);
+        if (i < n) store8<kAccess>(a.residual_out + row * a.width, 8 * i - shift, a.width, v[p]);
       }
     } else {
 #pragma unroll
@@ -145,12 +184,12 @@ add_rms_norm_kernel(const NormArgs a) {
     const int i = p * a.team + lane;
     if (i < n) {
       float w[8];
-      load_weight8<kVec>(a.weight, a.weight_f32, i, a.width, w);
+      load_weight8<kAccess>(a.weight, a.weight_f32, 8 * i - shift, shift, a.width, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[p][j] = __fmul_rn(__fmul_rn(v[p][j], rstd), w[j]);
-      if (a.y != nullptr) store8<kVec>(a.y + row * a.width, i, a.width, v[p]);
+      if (a.y != nullptr) store8<kAccess>(a.y + row * a.width, 8 * i - shift, a.width, v[p]);
     }
-    if (a.q != nullptr) {                // four lanes hold a block, sixteen the four blocks of a word of scales
+    if (kAccess != kShifted && a.q != nullptr) {       // four lanes hold a block, sixteen the four blocks of a word of scales
       uint32_t m = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[p][j]) & 0x7FFFFFFFu);
@@ -223,8 +262,10 @@ quant_mx8_kernel(const __nv_bfloat16* __restrict__ x, long long x_stride, unsign
 }
 
 template <int V>
-cudaError_t launch_norm(const NormArgs& a, bool vec, dim3 grid, dim3 block, cudaStream_t s) {
-  return launch_pdl(vec ? add_rms_norm_kernel<V, true> : add_rms_norm_kernel<V, false>, grid, block, 0, s, pdl_enabled(), a);
+cudaError_t launch_norm(const NormArgs& a, Access access, dim3 grid, dim3 block, cudaStream_t s) {
+  return launch_pdl(access == kWhole ? add_rms_norm_kernel<V, kWhole> : access == kShifted ? add_rms_norm_kernel<V, kShifted>
+                                                                                          : add_rms_norm_kernel<V, kSingle>,
+                    grid, block, 0, s, pdl_enabled(), a);
 }
 
 bool aligned_to(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -249,9 +290,12 @@ extern "C" int pnv_add_rms_norm(const void* x, int64_t x_stride, const void* res
   PNV_REQUIRE(aligned_to(x, 2) && aligned_to(residual, 2) && aligned_to(weight, weight_is_f32 ? 4 : 2) && aligned_to(y, 2) &&
                   aligned_to(residual_out, 2) && aligned_to(q, 8) && aligned_to(q_sf, 4),
               "add_rms_norm: a buffer is not aligned to its elements (codes 8 bytes, scales 4)");
-  const bool vec = width % 8 == 0 && x_stride % 8 == 0 && residual_stride % 8 == 0 && aligned_to(x, 16) && aligned_to(residual, 16) &&
-                   aligned_to(weight, 16) && aligned_to(y, 16) && aligned_to(residual_out, 16);
-  const int n = ceil_div_i(width, kVecElems);
+  // Whole 16-byte accesses; else shifted ones, where all rows lie alike within 16 bytes (odd widths, 8-bit output not among them);
+  // else element by element.  16384 x 4097, bf16 output and residual: 132 us shifted, 316 element by element (4096: 80 whole).
+  const bool aligned = aligned_to(x, 16) && aligned_to(residual, 16) && aligned_to(weight, 16) && aligned_to(y, 16) && aligned_to(residual_out, 16);
+  const bool alike = x_stride % 8 == width % 8 && (residual == nullptr || residual_stride % 8 == width % 8);
+  const Access access = !aligned || !alike ? kSingle : width % 8 == 0 ? kWhole : width + 7 <= PNV_NORM_MAX_WIDTH ? kShifted : kSingle;
+  const int n = ceil_div_i(width + (access == kShifted ? 7 : 0), kVecElems);
   if (sm_count <= 0) sm_count = 148;
   // Many rows: as few threads a row as hold it with five pieces each (16384 x 7168 with both outputs: 167 us; with seven 180,
   // the fewer rows of an SM are then not enough to keep memory busy while one of them is added up; with three 228).  Rows that
@@ -265,14 +309,14 @@ extern "C" int pnv_add_rms_norm(const void* x, int64_t x_stride, const void* res
   const dim3 grid((unsigned)blocks), block((unsigned)threads);
   cudaStream_t s = (cudaStream_t)stream;
   switch (ceil_div_i(n, team)) {
-    case 1: PNV_CUDA(launch_norm<1>(a, vec, grid, block, s)); break;
-    case 2: PNV_CUDA(launch_norm<2>(a, vec, grid, block, s)); break;
-    case 3: PNV_CUDA(launch_norm<3>(a, vec, grid, block, s)); break;
-    case 4: PNV_CUDA(launch_norm<4>(a, vec, grid, block, s)); break;
-    case 5: PNV_CUDA(launch_norm<5>(a, vec, grid, block, s)); break;
-    case 6: PNV_CUDA(launch_norm<6>(a, vec, grid, block, s)); break;
-    case 7: PNV_CUDA(launch_norm<7>(a, vec, grid, block, s)); break;
-    default: PNV_CUDA(launch_norm<8>(a, vec, grid, block, s)); break;
+    case 1: PNV_CUDA(launch_norm<1>(a, access, grid, block, s)); break;
+    case 2: PNV_CUDA(launch_norm<2>(a, access, grid, block, s)); break;
+    case 3: PNV_CUDA(launch_norm<3>(a, access, grid, block, s)); break;
+    case 4: PNV_CUDA(launch_norm<4>(a, access, grid, block, s)); break;
+    case 5: PNV_CUDA(launch_norm<5>(a, access, grid, block, s)); break;
+    case 6: PNV_CUDA(launch_norm<6>(a, access, grid, block, s)); break;
+    case 7: PNV_CUDA(launch_norm<7>(a, access, grid, block, s)); break;
+    default: PNV_CUDA(launch_norm<8>(a, access, grid, block, s)); break;
   }
   return PNV_OK;
 }

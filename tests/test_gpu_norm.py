@@ -40,7 +40,8 @@ def check_codes(q, sf, n, rows, width):
 
 # widths: one element, odd, just past a vector, the repository's hidden sizes, the largest; rows around atoms of 128
 @pytest.mark.parametrize("rows,width", [(1, 1), (3, 7), (2, 33), (5, 264), (129, 1023), (64, 2048), (31, 2880), (300, 2880), (1, 7168),
-                                        (2, 4096), (700, 4104), (130, 7168), (3, 16384), (400, 5120), (1, 32768), (301, 32768)])
+                                        (2, 4096), (700, 4104), (130, 7168), (3, 16384), (400, 5120), (1, 32768), (301, 32768),
+                                        (300, 4097), (9, 8191), (33, 2881), (5, 32761), (3, 32767), (40, 12), (2000, 1), (700, 9)])
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("weight_type", [torch.bfloat16, torch.float32])
 def test_norm_matches_64_bits(ops, rows, width, residual, weight_type):
@@ -75,6 +76,37 @@ def test_strided_rows(ops, rows, width, pad, offset):
     want = ops.add_rms_norm(x.contiguous(), r.contiguous(), w, 1e-5, True, True)
     for a, b in zip(got, want):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+# odd widths whose rows lie alike within 16 bytes in every buffer, and ones where they do not
+@pytest.mark.parametrize("pad,offset", [(8, 8), (64, 16), (1, 0), (8, 3)])
+@pytest.mark.parametrize("rows,width", [(5, 63), (200, 2881), (1, 97), (300, 4094)])
+@pytest.mark.parametrize("weight_type", [torch.bfloat16, torch.float32])
+def test_strided_rows_of_odd_widths(ops, rows, width, pad, offset, weight_type):
+    x, r = make(rows, width, 4, 1.0, pad + offset, offset), make(rows, width, 5, 1.0, pad + offset + 8, offset)
+    w = make(1, width, 6)[0].to(weight_type).contiguous()
+    got = ops.add_rms_norm(x, r, w, 1e-5)
+    want = ops.add_rms_norm(x.contiguous(), r.contiguous(), w, 1e-5)
+    v, n = ref.norm(x.cpu(), r.cpu(), w.cpu(), 1e-5)
+    for t in (got, want):
+        assert bool(((t[0].cpu().double() - n).abs() <= n.abs() * (BF16 + 2 * F32) + 1e-38).all())
+        assert torch.equal(t[1].cpu(), v.float().to(torch.bfloat16))
+
+
+def test_nothing_is_written_outside_of_odd_rows(ops):
+    """C entry on pieces of larger buffers: rows of 4097 elements, outputs with a guard on either side."""
+    from paired_nvfp4_kernels import _cabi
+    rows, width = 37, 4097
+    x, w = make(rows, width, 7).contiguous(), make(1, width, 8)[0].contiguous()
+    for lead in (8, 3):
+        bufs = [torch.full((rows * width + 64,), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        y, res = (b[lead:lead + rows * width].view(rows, width) for b in bufs)
+        rc = _cabi.lib.pnv_add_rms_norm(x.data_ptr(), width, x.data_ptr(), width, w.data_ptr(), 0, 1e-6, rows, width, y.data_ptr(), res.data_ptr(),
+                                        None, None, 0, torch.cuda.current_stream().cuda_stream)
+        want = ops.add_rms_norm(x, x, w)
+        off = (y.double() - want[0].double()).abs()            # (another grouping of the sum: a unit at most)
+        assert rc == 0 and bool((off <= want[0].double().abs() * 2 * BF16).all()) and torch.equal(res, want[1])
+        assert all(bool((b[:lead] == 7).all()) and bool((b[lead + rows * width:] == 7).all()) for b in bufs)
 
 
 def test_weight_at_an_odd_element(ops):
