@@ -61,7 +61,7 @@ struct LinearArgs {
   int out_f32, bias_f32, gated, kind;    // kind: PNV_ACT_*
   GatedAct act;
   int vec_out, vec_residual, vec_bias;   // may these be accessed 16 bytes at a time
-  int tma_out, tma_res;                  // pair kernel: do outputs leave and residuals come by TMA copies
+  int tma;                               // pair kernel: do outputs leave and residuals come by TMA copies
 };
 
 // What an epilogue does between bias and residual.  Kernels are compiled for each: with all the activations' code in one
@@ -553,7 +553,8 @@ template <bool kMx8, int kMode>
 __global__ void __launch_bounds__(PairCfg<kMx8>::kThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const __grid_constant__ CUtensorMap map_w_sf, const __grid_constant__ CUtensorMap map_x_sf,
-                   const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_res, const LinearArgs a) {
+                   const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_out_32,
+                   const __grid_constant__ CUtensorMap map_res, const __grid_constant__ CUtensorMap map_res_32, const LinearArgs a) {
   using C = PairCfg<kMx8>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
@@ -670,21 +671,23 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     }
   } else if (warp >= 2) {
     // ---- epilogue: a tile's blocks of 64 features go to the two groups in turn, a thread has one token's.  Outputs leave and
-    // residuals come through 4 KB of shared memory per warp and TMA copies of 32 tokens x 32 features (64-byte swizzle), a
-    // thread reading its residuals from where it puts its outputs.  With loads and stores of its own, 32 rows apart from lane
-    // to lane, the epilogue of a tile with a residual took 10000 cycles, where the products of K = 2048 take 8200.
+    // residuals come through 4 KB of shared memory per warp and TMA copies of 32 tokens x 64 features (128-byte swizzle; of 32
+    // features, 64-byte swizzle, where a tile ends with them or gates leave half), a thread reading its residuals from where it
+    // puts its outputs.  With loads and stores of its own, 32 rows apart from lane to lane, the epilogue of a tile with a residual
+    // took 10000 cycles, where the products of K = 2048 take 8200.  What copies cannot take goes the other way (slow).
     const int quarter = warp & 3, group = (warp - 2) >> 2;
     uint8_t* mine = staging + (warp - 2) * 4096;
-    const bool staged_res = a.residual != nullptr && a.tma_res != 0;
+    const bool staged_res = a.residual != nullptr && a.tma != 0;
     int acc = 0;
     uint32_t acc_phase = 0, res_phase = 0;
     bool ok = true;
+    const auto is_wide = [&](int block) { return kMode != kGate && a.tile_n - block * 64 >= 64; };
     // The residual of a block of a tile (tokens from row0 on) is asked for; lane 0, whose stores from there have been read.
-    auto ask = [&](int row0, int nt, int block) {
-      const int col = nt * a.tile_n + block * 64, out0 = kMode == kGate ? col / 2 : col;
-      ptx::mbar_arrive_expect_tx(res_full + warp - 2, kMode == kGate ? 2048 : 4096);
-      ptx::tma_load_3d(mine, &map_res, res_full + warp - 2, out0, row0, 0);
-      if (kMode != kGate) ptx::tma_load_3d(mine + 2048, &map_res, res_full + warp - 2, out0 + 32, row0, 0);
+    const auto ask = [&](int row0, int nt, int block) {
+      const int col = nt * a.tile_n + block * 64;
+      const bool wide = is_wide(block);
+      ptx::mbar_arrive_expect_tx(res_full + warp - 2, wide ? 4096 : 2048);
+      ptx::tma_load_3d(mine, wide ? &map_res : &map_res_32, res_full + warp - 2, kMode == kGate ? col / 2 : col, row0, 0);
     };
     const int last_blocks = (a.tile_n + 63) / 64;
     if (staged_res && group < last_blocks && (int)blockIdx.x / 2 < tiles && lane == 0) {
@@ -740,7 +743,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             continue;
           }
           res_phase ^= 1;
-        } else if (a.tma_out) {
+        } else if (a.tma) {
           if (lane == 0) ptx::bulk_wait_read_all();
           __syncwarp();
         }
@@ -751,51 +754,60 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             r[i][1][j] = __float_as_uint(__uint_as_float(r[i][1][j]) + __shfl_sync(0xffffffffu, bias[i][1], j));
           }
         }
+        const bool wide = is_wide(block);
+        if (__builtin_expect(a.tma, 1)) {
+          // this thread's row of the box, 16-byte pieces swizzled by the row (what lies past the matrix is not copied out)
+          uint8_t* line = mine + lane * (wide ? 128 : 64);
+          const int swz = wide ? lane & 7 : (lane >> 1) & 3;
 #pragma unroll
-        for (int h = 0; h < 64; h += 16) {
-          if (kMode == kGate ? h >= 32 || 2 * h >= width : h >= width) continue;      // (gated: a whole block or nothing)
-          float v[16];
-          if constexpr (kMode == kGate) {
-            if (h < 32) {
-              float g[16], u[16];
+          for (int h = 0; h < (kMode == kGate ? 32 : 64); h += 8) {
+            if (kMode != kGate && h == 32 && !wide) break;
+            float v[8];
+            if constexpr (kMode == kGate) {
+              float g[8], u[8];
 #pragma unroll
-              for (int j = 0; j < 16; ++j) { g[j] = __uint_as_float(r[i][0][h % 32 + j]); u[j] = __uint_as_float(r[i][1][h % 32 + j]); }
+              for (int j = 0; j < 8; ++j) { g[j] = __uint_as_float(r[i][0][h + j]); u[j] = __uint_as_float(r[i][1][h + j]); }
               gate(g, u, v, a);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[i][h / 32][h % 32 + j]);
+              if constexpr (kMode == kActivate) activate(v, a);
             }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[i][h / 32][h % 32 + j]);
-            if constexpr (kMode == kActivate) activate(v, a);
-          }
-          // this thread's row of the box, 16-byte pieces swizzled by the row
-          uint4* line = reinterpret_cast<uint4*>(mine + (h / 32) * 2048 + lane * 64);
-          const int swz = (lane >> 1) & 3, piece = (h % 32) / 8;
-          if (staged_res) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            uint4* at = reinterpret_cast<uint4*>(line + (((h / 8) ^ swz) << 4));
+            if (staged_res) {
               float f[8];
-              unpack8(line[(piece + j) ^ swz], f);
+              unpack8(*at, f);
 #pragma unroll
-              for (int q = 0; q < 8; ++q) v[8 * j + q] += f[q];
+              for (int j = 0; j < 8; ++j) v[j] += f[j];
             }
+            *at = make_uint4(as_u32(__floats2bfloat162_rn(v[0], v[1])), as_u32(__floats2bfloat162_rn(v[2], v[3])),
+                             as_u32(__floats2bfloat162_rn(v[4], v[5])), as_u32(__floats2bfloat162_rn(v[6], v[7])));
           }
-          if (a.tma_out) {
-            if (!staged_res && a.residual != nullptr && row < a.rows) add_residual(v, a, row, out_col + h);
+          ptx::fence_proxy_async_smem();
+        } else if (row < a.rows) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              line[(piece + j) ^ swz] = make_uint4(as_u32(__floats2bfloat162_rn(v[8 * j], v[8 * j + 1])), as_u32(__floats2bfloat162_rn(v[8 * j + 2], v[8 * j + 3])),
-                                                   as_u32(__floats2bfloat162_rn(v[8 * j + 4], v[8 * j + 5])), as_u32(__floats2bfloat162_rn(v[8 * j + 6], v[8 * j + 7])));
-          } else if (row < a.rows) {
-            if (!staged_res) add_residual(v, a, row, out_col + h);
-            store_outputs(v, a, row, out_col + h);
+          for (int h = 0; h < (kMode == kGate ? 32 : 64); h += 8) {
+            if (h < width) {             // (gated: a whole block or nothing)
+              float v[8];
+              if constexpr (kMode == kGate) {
+                float g[8], u[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { g[j] = __uint_as_float(r[i][0][h + j]); u[j] = __uint_as_float(r[i][1][h + j]); }
+                gate(g, u, v, a);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[i][h / 32][h % 32 + j]);
+                if constexpr (kMode == kActivate) activate(v, a);
+              }
+              add_residual(v, a, row, out_col + h);
+              store_outputs(v, a, row, out_col + h);
+            }
           }
         }
-        if (a.tma_out) ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          if (a.tma_out && row0 < a.rows && width > 0) {
-            ptx::tma_store_3d(&map_out, mine, out_col, row0, 0);
-            if (kMode != kGate && width > 32) ptx::tma_store_3d(&map_out, mine + 2048, out_col + 32, row0, 0);
+          if (a.tma && row0 < a.rows && width > 0) {
+            ptx::tma_store_3d(wide ? &map_out : &map_out_32, mine, out_col, row0, 0);
             ptx::bulk_commit();
           }
           if (staged_res) {              // the next block's residual, once the copies have read this one's outputs
@@ -854,10 +866,10 @@ int scale_map(CUtensorMap* map, const void* base, uint64_t row_atoms, uint64_t k
   return make_view(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 128, k_atoms, 512, 128, 1, CU_TENSOR_MAP_SWIZZLE_NONE,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, row_atoms, atoms);
 }
-// bf16 rows, `stride` elements apart, in boxes of 32 x 32 (64-byte swizzle): outputs and residuals.
-int rows_map(CUtensorMap* map, const void* base, uint64_t width, uint64_t rows, uint64_t stride) {
-  return make_view(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, width, rows, stride * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B,
-                   CU_TENSOR_MAP_L2_PROMOTION_NONE);
+// bf16 rows, `stride` elements apart, in boxes of 64 or 32 columns x 32 rows (128- or 64-byte swizzle): outputs and residuals.
+int rows_map(CUtensorMap* map, const void* base, uint64_t width, uint64_t rows, uint64_t stride, uint32_t box) {
+  return make_view(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, width, rows, stride * 2, box, 32,
+                   box == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE);
 }
 
 constexpr int kMaxSplitLog = 3;          // clusters of 1, 2, 4 or 8 CTAs
@@ -1014,7 +1026,7 @@ int launch_pair(const Operands& o, LinearArgs a, int width, int sm_count, cudaSt
   a.band = kLowBand;
   while (a.band < kHighBand && 2LL * a.band * 256 * a.k_bytes <= kBandBytes) a.band *= 2;
   const int pairs = std::min(sm_count / 2, a.m_tiles * a.n_tiles);
-  CUtensorMap map_w, map_x, map_w_sf = {}, map_x_sf = {}, map_out = {}, map_res = {};
+  CUtensorMap map_w, map_x, map_w_sf = {}, map_x_sf = {};
   if (int rc = operand_map(&map_w, o.w, a.k_bytes, a.features, a.k_bytes, a.tile_n / 2)) return rc;
   if (int rc = operand_map(&map_x, o.x, a.k_bytes, a.rows, o.x_stride, 128)) return rc;
   if (kMx8) {
@@ -1022,14 +1034,18 @@ int launch_pair(const Operands& o, LinearArgs a, int width, int sm_count, cudaSt
     if (int rc = scale_map(&map_w_sf, a.w_sf, sf_row_atoms(a.features), k_atoms, 2)) return rc;
     if (int rc = scale_map(&map_x_sf, a.x_sf, sf_row_atoms(a.rows), k_atoms, 1)) return rc;
   }
-  a.tma_out = a.vec_out;
-  a.tma_res = a.tma_out && a.residual != nullptr && a.vec_residual;
-  if (a.tma_out)
-    if (int rc = rows_map(&map_out, a.out, a.n_out, a.rows, a.n_out)) return rc;
-  if (a.tma_res)
-    if (int rc = rows_map(&map_res, a.residual, a.n_out, a.rows, a.residual_stride)) return rc;
+  a.tma = a.vec_out && (a.residual == nullptr || a.vec_residual);
+  CUtensorMap map_out = {}, map_out_32 = {}, map_res = {}, map_res_32 = {};
+  if (a.tma) {
+    if (int rc = rows_map(&map_out, a.out, a.n_out, a.rows, a.n_out, 64)) return rc;
+    if (int rc = rows_map(&map_out_32, a.out, a.n_out, a.rows, a.n_out, 32)) return rc;
+    if (a.residual != nullptr) {
+      if (int rc = rows_map(&map_res, a.residual, a.n_out, a.rows, a.residual_stride, 64)) return rc;
+      if (int rc = rows_map(&map_res_32, a.residual, a.n_out, a.rows, a.residual_stride, 32)) return rc;
+    }
+  }
   PNV_CUDA(launch_clusters(linear_pair_kernel<kMx8, kMode>, dim3((unsigned)(2 * pairs)), C::kThreads, C::kSmem, 2, stream, map_w, map_x, map_w_sf,
-                           map_x_sf, map_out, map_res, a));
+                           map_x_sf, map_out, map_out_32, map_res, map_res_32, a));
   return PNV_OK;
 }
 
