@@ -15,7 +15,7 @@
 // and residual, in parentheses):
 //   pair     the tensor pipe, and above a few hundred microseconds the power limit: 8192 x 28672 x 4096 gated 1150 us, 1.67
 //            PFLOP/s, tensor pipe 89 % busy (1190); the same in a loop of seconds 1350 us (1390).  8-bit operands: 8192 x 7168 x
-//            2048 91 us (84), with a residual 104; in a loop 108 and 124 (103).
+//            2048 88 us (84), with a residual 100; in a loop 107 and 120 (103).
 //   split    latency where little is read: 16 x 256 x 7168 to float32 4.7 us (10.7); what a CTA takes in, 85 bytes a cycle, and
 //            the way of the partial sums, 16 bytes a cycle, otherwise: 64 x 4096 x 7168 gated on 8-bit operands 8.4 us, 30 MB
 //            (12.9).
@@ -923,7 +923,7 @@ int cluster_capacity(const int** out) {
 //
 // The constants are a fit, in units of 1/1.9 ns, to measured times of all the candidates for eight weights from 256 x 7168 to
 // 28672 x 4096 and 1 to 4096 tokens, both operand types (two thousand calls): off by a tenth on average; the candidate that it
-// picks is 1.1 % slower than the best one on average and 18 % at worst.
+// picks is 1.3 % slower than the best one on average and 19 % at worst.
 
 struct Plan {
   int tokens;                            // split kernel: tokens of a tile; 0: pair kernel

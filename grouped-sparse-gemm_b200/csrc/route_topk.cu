@@ -7,7 +7,7 @@
 // A warp takes a token: its keys lie in registers as unsigned numbers that order like them, every round of the selection is
 // two warp-wide integer reductions (largest key, lowest expert that has it).  Keys with a bias are sums of 32-bit roundings,
 // so two that lie closer together than those can be off might come out in the wrong order: where a selected key is that
-// close to the next one, the row is done again in 64 bits (a handful of rows in a thousand at 256 experts).
+// close to the next one, the row is done again in 64 bits (a row in a thousand at 256 experts).
 // Bound: issue slots for many rows (16384 x 128, top-8 of softmax: 10.7 us, 554 instructions a row, 77 % of the slots), latency of
 // the reductions for few (64 x 256, top-8 of sigmoid with bias, 4 of 8 groups: 7.2 us).  One kernel for all options, keys found
 // anew every round, took 15.6 us for the former.
@@ -87,11 +87,12 @@ __device__ __forceinline__ F softmax_sum(const RouteArgs& a, const void* row, in
   return sum;
 }
 
-// Are two neighbouring keys, the larger one first, too close for 32 bits to order?  A sigmoid is off by at most 2e-7 (2^-22 of
-// the exponential, times s (1 - s), and the reciprocal's unit), a softmax by 1.5e-6 (its sum over 1024), the sum with the bias
-// by half a unit more; a group's sum of two by twice that.
-__device__ __forceinline__ bool too_close(float larger, float smaller, float terms, bool sigmoid) {
-  return larger - smaller <= terms * (sigmoid ? 9.5367432e-7f : 3.8146973e-6f) * (1.f + fabsf(larger));
+// Two neighbouring keys, the larger one first, are too close for 32 bits to order where their difference is within what both can
+// be off.  A sigmoid is off by 1.2e-7 (the largest of 2^31 values between -100 and 100 against 64 bits), a softmax by 1.5e-6 (its
+// sum over 1024), the sum with the bias by half a unit, 6e-8 of the key; a group's sum of two keys by twice that, of either key,
+// and half a unit of its own.  large: the largest magnitude among them.
+__device__ __forceinline__ bool too_close(float larger, float smaller, float terms, float large, bool sigmoid) {
+  return larger - smaller <= terms * (sigmoid ? fmaf(1.5e-7f, large, 3e-7f) : fmaf(3.8e-6f, large, 3.8e-6f));
 }
 
 // Lane r < topk returns expert r of the row, best first, and its key; logit[j] is that of expert 32 j + lane.  doubtful: (32 bits
@@ -121,6 +122,7 @@ __device__ __forceinline__ int select(const RouteArgs& a, const void* row, const
   if constexpr (kGroups) {
     O mine = 0;                          // lane g: the score of group g
     int g = 0;
+    float large = 0.f;                   // the largest magnitude of a group's best
     O first = 0, second = 0;             // this lane's two best of a group
     auto take = [&](O k) {
       if (kBias) second = max(second, min(first, k));
@@ -133,6 +135,7 @@ __device__ __forceinline__ int select(const RouteArgs& a, const void* row, const
         const int owner = __ffs(__ballot_sync(kAll, first == best)) - 1;
         const O next = warp_max(lane == owner ? second : first);
         score = next == 0 ? best : order_of(key_of(best) + key_of(next));
+        if (kCheck && fabsf((float)key_of(best)) < INFINITY) large = fmaxf(large, fabsf((float)key_of(best)));
       }
       if (lane == g) mine = score;
       first = second = 0;
@@ -158,7 +161,7 @@ __device__ __forceinline__ int select(const RouteArgs& a, const void* row, const
     for (int r = 0; r <= a.topk_groups && r < a.groups; ++r) {
       const O best = warp_max(mine);
       if (r == a.topk_groups) {          // (the order among the kept does not matter, only the border)
-        if (kCheck) doubtful |= too_close((float)last, (float)key_of(best), 2.f, a.sigmoid);
+        if (kCheck) doubtful |= too_close((float)last, (float)key_of(best), 2.f, large + fabsf((float)last), a.sigmoid);
         break;
       }
       const int chosen = __ffs(__ballot_sync(kAll, mine == best && lane < a.groups)) - 1;
@@ -221,7 +224,7 @@ __device__ __forceinline__ int select(const RouteArgs& a, const void* row, const
     }
     if (kCheck) {
       const F k = key_of(best);
-      if (r > 0) doubtful |= too_close((float)last, (float)k, 1.f, a.sigmoid);
+      if (r > 0) doubtful |= too_close((float)last, (float)k, 1.f, fabsf((float)last), a.sigmoid);
       last = k;
     }
     if (lane == r) { picked = e; picked_key = best; }

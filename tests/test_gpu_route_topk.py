@@ -66,6 +66,19 @@ def test_keys_closer_than_32_bits_can_order(ops):
     check(ops, logits, 8, "softmax", torch.randn(64, generator=g).mul(1e-9).cuda(), 4, 3)
 
 
+@pytest.mark.parametrize("spread", [1e-6, 3e-7, 1e-7, 2e-8])
+@pytest.mark.parametrize("offset", [0.0, 4.0, -4.0])
+def test_keys_around_the_doubt(ops, spread, offset):
+    """Keys whose differences are about as large as the error of 32 bits, at several magnitudes of the bias, cancelling ones too."""
+    g = torch.Generator().manual_seed(11)
+    logits = make(400, 64, 12)
+    base = offset * torch.where(torch.arange(64) % 2 == 0, 1.0, -1.0)
+    bias = (base.double() - torch.sigmoid(logits[0].cpu().double()) + spread * torch.randn(64, generator=g).double()).float().cuda()
+    rows = logits[:1].expand(400, 64) + torch.randn((400, 64), generator=g).cuda() * spread
+    check(ops, rows.contiguous(), 8, "sigmoid", bias)
+    check(ops, rows.contiguous(), 8, "sigmoid", bias, 8, 4)
+
+
 def test_rows_of_infinities_and_nan(ops):
     inf, nan = math.inf, math.nan
     logits = torch.tensor([[-inf] * 8, [-inf, 1, -inf, 2, -inf, -inf, -inf, -inf], [nan, 1, 2, 3, 4, 5, nan, 7], [inf, 1, inf, 2, 3, 4, 5, 6],
