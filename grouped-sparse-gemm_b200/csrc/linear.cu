@@ -442,6 +442,19 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     }
   }
   __syncwarp();
+  // Outputs are made in pieces of eight neighbouring features of a token; a thread's pieces have the same features.  Gated:
+  // features [64 b, 64 b + 32) are gates, the next 32 their ups.
+  constexpr int kPieces = kMode == kGate ? 8 : 16;
+  static_assert(C::kThreads % kPieces == 0, "a thread keeps its features from token to token");
+  const int piece = (int)threadIdx.x % kPieces;
+  const int f = kMode == kGate ? (piece >> 2) * 64 + (piece & 3) * 8 : piece * 8, col = ft * kTileRows + f;
+  float bias[8], up_bias[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) bias[j] = up_bias[j] = 0.f;
+  if (col < a.features) {
+    add_bias(bias, a, col);
+    if (kMode == kGate) add_bias(up_bias, a, col + 32);
+  }
   ptx::tc_fence_before();
   if (split > 1) {
     if (warp < 4) ptx::cluster_wait();
@@ -463,41 +476,41 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     ptx::tmem_dealloc(tmem, C::kTmemCols);
   }
 
-  // ---- this CTA's share of the tile's outputs, in pieces of eight neighbouring features of a token
-  const int per_token = kMode == kGate ? 8 : 16;
-  for (int u = (int)threadIdx.x; u < own * per_token; u += C::kThreads) {
-    const int token = u / per_token, piece = u - token * per_token;
-    // gated: features [64 b, 64 b + 32) are gates, the next 32 their ups
-    const int f = kMode == kGate ? (piece >> 2) * 64 + (piece & 3) * 8 : piece * 8;
-    const int col = ft * kTileRows + f, row = tt * BN + rank * share + token;
-    if (col >= a.features) continue;
-    float v[8], up[8];
+  // ---- this CTA's share of the tile's outputs
+  if (col < a.features) {
+    const int out_col = kMode == kGate ? (col - f) / 2 + (piece >> 2) * 32 + (piece & 3) * 8 : col;
+#pragma unroll(kMode == kGate ? 1 : 2)
+    for (int token = (int)threadIdx.x / kPieces; token < own; token += C::kThreads / kPieces) {
+      const int row = tt * BN + rank * share + token;
+      float v[8], up[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = up[j] = 0.f;
-    const float4* src = reinterpret_cast<const float4*>(sums + token * kTileRows + f);
+      for (int j = 0; j < 8; ++j) v[j] = up[j] = 0.f;
+      const float4* src = reinterpret_cast<const float4*>(sums + token * kTileRows + f);
 #pragma unroll 4
-    for (int r = 0; r < split; ++r, src += share * (kTileRows / 4)) {
-      const float4 p = src[0], q = src[1];
-      v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
-      v[4] += q.x; v[5] += q.y; v[6] += q.z; v[7] += q.w;
-      if constexpr (kMode == kGate) {
-        const float4 s = src[8], t = src[9];
-        up[0] += s.x; up[1] += s.y; up[2] += s.z; up[3] += s.w;
-        up[4] += t.x; up[5] += t.y; up[6] += t.z; up[7] += t.w;
+      for (int r = 0; r < split; ++r, src += share * (kTileRows / 4)) {
+        const float4 p = src[0], q = src[1];
+        v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
+        v[4] += q.x; v[5] += q.y; v[6] += q.z; v[7] += q.w;
+        if constexpr (kMode == kGate) {
+          const float4 s = src[8], t = src[9];
+          up[0] += s.x; up[1] += s.y; up[2] += s.z; up[3] += s.w;
+          up[4] += t.x; up[5] += t.y; up[6] += t.z; up[7] += t.w;
+        }
       }
-    }
-    add_bias(v, a, col);
-    if constexpr (kMode == kGate) {
-      add_bias(up, a, col + 32);
-      float y[8];
-      gate(v, up, y, a);
-      const int out_col = (col - f) / 2 + (piece >> 2) * 32 + (piece & 3) * 8;
-      add_residual(y, a, row, out_col);
-      store_outputs(y, a, row, out_col);
-    } else {
-      if constexpr (kMode == kActivate) activate(v, a);
-      add_residual(v, a, row, col);
-      store_outputs(v, a, row, col);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += bias[j];
+      if constexpr (kMode == kGate) {
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) up[j] += up_bias[j];
+        gate(v, up, y, a);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = y[j];
+      } else if constexpr (kMode == kActivate) {
+        activate(v, a);
+      }
+      add_residual(v, a, row, out_col);
+      store_outputs(v, a, row, out_col);
     }
   }
   if (split > 1) ptx::cluster_wait();    // what this CTA sent has arrived: its memory may go
