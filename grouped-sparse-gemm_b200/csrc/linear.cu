@@ -520,8 +520,8 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 //
 // Six stages of 32 KB (8-bit operands: five of 34 KB with the scales) beside 32 KB in which residuals arrive and outputs leave:
 // with twice that for the epilogue and a stage less the products waited (8192 x 7168 x 2048: 83 us instead of 77).  Eight
-// epilogue warps: a thread keeps its 128 accumulators in registers, so that the one accumulator of 8-bit operands (the scale
-// words need the other's columns) is free again after 130 cycles.
+// epilogue warps: a thread keeps its 128 accumulators in registers, so that where there is one accumulator (8-bit operands and
+// tiles of 256 features: the scale words need the other's columns) it is free again after 130 cycles.
 
 template <bool kMx8>
 struct PairCfg {
@@ -533,13 +533,16 @@ struct PairCfg {
   static constexpr int kStageBytes = kABytes + kBBytes + (kMx8 ? 2048 : 0);
   static constexpr int kStagingBytes = kEpiWarps * 4096;             // a warp's 32 tokens x 64 features of residual and output
   static constexpr int kStages = (kSmemMax - 1024 - kBarBytes - kStagingBytes) / kStageBytes;
-  // 8-bit operands: the scale words need columns, so there is one accumulator; its readers hand it back as soon as they
-  // have it in registers
-  static constexpr int kAccs = kMx8 ? 1 : 2;
-  static constexpr int kColSf = kAccs * kTileN;
+  // Two accumulators, so that a tile's products are made while the one before is read.  8-bit operands: the scale words need
+  // columns too, so there are two of up to 192 features, or one; its readers hand it back as soon as they have it in registers.
+  // (Tiles of 192 in several waves, two against one: 2048 x 7168 x 2048 25.4 us against 26.6, with a residual 27.4 against 29.1.)
+  static constexpr int kAccWidth = kMx8 ? 192 : kTileN;
   static constexpr int kTmemCols = 512;
+  __host__ __device__ static constexpr int accs(int tile_n) { return tile_n <= kAccWidth ? 2 : 1; }
+  __host__ __device__ static constexpr int col_sf(int tile_n) { return tile_n <= kAccWidth ? 2 * kAccWidth : kTileN; }
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kStagingBytes + kBarBytes;
-  static_assert(kColSf + (kMx8 ? 12 * kStages : 0) <= kTmemCols, "tensor-memory column map overflows");
+  static_assert(col_sf(kAccWidth) + (kMx8 ? 12 * kStages : 0) <= kTmemCols && col_sf(kTileN) + (kMx8 ? 12 * kStages : 0) <= kTmemCols,
+                "tensor-memory column map overflows");
 };
 
 // Tiles in bands along the tokens, features outer within a band: the tiles that run at one time share activations and weights
@@ -575,8 +578,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   uint64_t* full = reinterpret_cast<uint64_t*>(staging + C::kStagingBytes);
   uint64_t* empty = full + C::kStages;
   uint64_t* acc_full = empty + C::kStages;
-  uint64_t* acc_empty = acc_full + C::kAccs;
-  uint64_t* res_full = acc_empty + C::kAccs;                           // one per epilogue warp
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* res_full = acc_empty + 2;                                  // one per epilogue warp
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + C::kEpiWarps);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = ptx::cluster_ctarank();
@@ -588,7 +591,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         ptx::mbar_init(full + s, 1);
         ptx::mbar_init(empty + s, 1);
       }
-      for (int b = 0; b < C::kAccs; ++b) {
+      for (int b = 0; b < 2; ++b) {
         ptx::mbar_init(acc_full + b, 1);
         ptx::mbar_init(acc_empty + b, 2 * C::kEpiWarps);
       }
@@ -609,6 +612,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 
   const int k_stages = (a.k_bytes + kStageRow - 1) / kStageRow;
   const int tiles = a.m_tiles * a.n_tiles, pairs = (int)gridDim.x / 2;
+  const int accs = C::accs(a.tile_n);
   if (warp == 0) {
     // ---- producer, in both CTAs: own tokens, own half of the features; completion is counted on the first CTA's barrier
     int stage = 0;
@@ -665,14 +669,14 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         ptx::tc_fence_after();
         const uint32_t st = ptx::smem_u32(stages + stage * C::kStageBytes);
         if (ptx::elect_one()) {
-          const uint32_t sfa = tmem + C::kColSf + 12 * stage, sfb = sfa + 4;
+          const uint32_t sfa = tmem + C::col_sf(a.tile_n) + 12 * stage, sfb = sfa + 4;
           if constexpr (kMx8) {
             const uint32_t sf = st + kABytes + C::kBBytes;
             ptx::tc_cp_32x128b_warpx4<2>(sfa, ptx::smem_desc(sf, 128, 0, 0));
             ptx::tc_cp_32x128b_warpx4<2>(sfb, ptx::smem_desc(sf + 512, 128, 0, 0));
             ptx::tc_cp_32x128b_warpx4<2>(sfb + 4, ptx::smem_desc(sf + 1024, 128, 0, 0));
           }
-          issue_stage<2, kMx8>(tmem + acc * C::kTileN, ptx::smem_desc(st, 1024, 16, 2), ptx::smem_desc(st + kABytes, 1024, 16, 2), idesc,
+          issue_stage<2, kMx8>(tmem + acc * C::kAccWidth, ptx::smem_desc(st, 1024, 16, 2), ptx::smem_desc(st + kABytes, 1024, 16, 2), idesc,
                                stage_mmas(a.k_bytes, ks), ks == 0, sfa, sfb + sfb_shift);
           ptx::tc_commit_pair(empty + stage);
           if (ks + 1 == k_stages) ptx::tc_commit_pair(acc_full + acc);
@@ -680,7 +684,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         __syncwarp();
         if (++stage == C::kStages) { stage = 0; phase ^= 1; }
       }
-      if (++acc == C::kAccs) { acc = 0; acc_phase ^= 1; }
+      if (++acc == accs) { acc = 0; acc_phase ^= 1; }
     }
   } else if (warp >= 2) {
     // ---- epilogue: a tile's blocks of 64 features go to the two groups in turn, a thread has one token's.  Outputs leave and
@@ -733,7 +737,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       uint32_t r[2][2][32];              // (columns past the tile hold whatever they hold and are not used)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t src = tmem + ((uint32_t)quarter << 21) + acc * C::kTileN + (group + 2 * i) * 64;
+        const uint32_t src = tmem + ((uint32_t)quarter << 21) + acc * C::kAccWidth + (group + 2 * i) * 64;
         ptx::tc_ld_32x32(src, r[i][0]);
         ptx::tc_ld_32x32(src + 32, r[i][1]);
       }
@@ -741,7 +745,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive_cluster(acc_empty + acc, 0);
-      if (++acc == C::kAccs) { acc = 0; acc_phase ^= 1; }
+      if (++acc == accs) { acc = 0; acc_phase ^= 1; }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int block = group + 2 * i, col = nt * a.tile_n + block * 64, out_col = kMode == kGate ? col / 2 : col;
