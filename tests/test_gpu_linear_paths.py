@@ -43,6 +43,15 @@ def test_sizes_between_the_variants(ops, t, n, k, mx8):  # noqa: F811
         run(ops, t, n, k, mx8=mx8, gated=True, activation="silu", residual=True, seed=n + 1)
 
 
+# 8-bit operands, several tiles a pair of CTAs: with two accumulators (192 features) and with one (256)
+@pytest.mark.parametrize("t,n,k,width", [(1056, 4096, 2048, 192), (4674, 2048, 768, 192), (834, 5120, 2048, 192), (1550, 2880, 512, 192), (4096, 4096, 1024, 256)])
+def test_accumulators_in_turn(ops, t, n, k, width):  # noqa: F811
+    assert plan(t, n, k, mx8=True) == ("pair", width) and -(-t // 256) * -(-n // width) > 74
+    for residual in (False, True):
+        run(ops, t, n, k, mx8=True, residual=residual, seed=t)
+    run(ops, t, n, k, mx8=True, bias=torch.float32, activation="gelu", seed=t + 1)
+
+
 # weights that come from memory, not from L2: the copies of a stage ring land out of order
 @pytest.mark.parametrize("t", [8, 32, 40, 128, 300])
 @pytest.mark.parametrize("mx8", [False, True])
