@@ -68,15 +68,20 @@ __device__ __forceinline__ double sigmoid_of(double l) { return 1.0 / (1.0 + exp
 __device__ __forceinline__ float exp_of(float v) { return expf(v); }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
 
-// exp(l - mx), 1 where the two are the same infinity, 0 everywhere in a row of nothing but -infinity.
+// exp(l - mx), 1 where the two are the same infinity, 0 everywhere in a row of nothing but -infinity; NaN where either is one.
 template <class F>
 __device__ __forceinline__ F softmax_part(F l, F mx) { return mx == (F)-INFINITY ? (F)0 : l == mx ? (F)1 : exp_of(l - mx); }
 
+// The largest logit.  A NaN does not count beside a number, but where nothing is above -infinity it is the answer, so that all
+// scores of the row are NaN: as -infinity it would give the row the zeros of one that was masked.
 __device__ __forceinline__ float row_max(const RouteArgs& a, const void* row, int lane) {
   uint32_t m = 0;
   for (int e = lane; e < a.experts; e += 32) m = max(m, order_of(logit_at(a, row, e)));
   m = warp_max(m);
-  return m == 1u ? -INFINITY : key_of(m);
+  if (m > order_of(-INFINITY)) return key_of(m);
+  bool nan = false;
+  for (int e = lane; e < a.experts; e += 32) nan |= isnan(logit_at(a, row, e));
+  return __any_sync(kAll, nan) ? __uint_as_float(0x7FFFFFFFu) : -INFINITY;
 }
 template <class F>
 __device__ __forceinline__ F softmax_sum(const RouteArgs& a, const void* row, int lane, F mx) {
@@ -275,13 +280,9 @@ route_topk_kernel(const RouteArgs a) {
     if (a.sigmoid) {
       if (lane < a.topk) w = __fdiv_rn(1.f, 1.f + expf(-mine));
     } else {
-      float mx;                          // without bias and groups the first choice has it (a NaN is there only if all are)
-      if (!kBias && !kGroups) {
-        mx = __shfl_sync(kAll, mine, 0);
-        if (mx != mx) mx = -INFINITY;
-      } else {
-        mx = row_max(a, row, lane);
-      }
+      float mx = -INFINITY;              // without bias and groups the first choice has it, if it is a number
+      if (!kBias && !kGroups) mx = __shfl_sync(kAll, mine, 0);
+      if (kBias || kGroups || !(mx > -INFINITY)) mx = row_max(a, row, lane);
       if (lane < a.topk) w = softmax_part(mine, mx);
       if (!a.renormalize) {
         const float total = softmax_sum<float>(a, row, lane, mx);
