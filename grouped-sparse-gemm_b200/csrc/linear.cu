@@ -72,6 +72,22 @@ enum Mode : int { kNothing = 0, kActivate = 1, kGate = 2 };
 
 __device__ __forceinline__ float silu_f32(float g) { return g * rcp_approx(1.f + ex2_approx(g * -kLog2e)); }
 
+// v / 2 erfc(-v / sqrt(2)).  In 1 + erf a negative v cancels (6 % off at -5, nothing left from -6).  With a = |v|, t = 1 / (1 + 0.35 a):
+// erfc(a / sqrt(2)) / 2 = exp(-a^2 / 2) t Q(t), where t Q(t) is smooth; Q is its polynomial of degree 8 with the smallest
+// relative error over a < 14.5 (weighted least squares, 3.2e-8), above which the exponential is 0.  Off by 10 + v^2 units of 2^-23 at
+// most (v^2 / 2: what the exponent's rounding does).  4096 x 8192 x 4096 180 us, 1 + erff 178, erfcf 226.
+__device__ __forceinline__ float gelu_f32(float v) {
+  const float a = fabsf(v) > 16.f ? 16.f : fabsf(v);           // (an infinity would meet a zero; a NaN stays one)
+  const float t = rcp_approx(fmaf(a, 0.35f, 1.f));
+  constexpr float kQ[9] = {0.139621302f, 0.139863536f, 0.119821183f, 0.105552927f, -0.023213394f, 0.159321249f, -0.255840391f, 0.144031614f,
+                           -0.0291580297f};
+  float q = kQ[8];
+#pragma unroll
+  for (int i = 7; i >= 0; --i) q = fmaf(q, t, kQ[i]);
+  const float y = a * (t * q) * ex2_approx(a * a * (-0.5f * kLog2e));
+  return v > 0.f ? v - y : -y;
+}
+
 template <int E>
 __device__ __forceinline__ void add_bias(float (&v)[E], const LinearArgs& a, int col) {
   if (a.bias == nullptr) return;
@@ -125,7 +141,7 @@ __device__ __forceinline__ void activate(float (&v)[E], const LinearArgs& a) {
       break;
     case PNV_ACT_GELU:
 #pragma unroll
-      for (int j = 0; j < E; ++j) v[j] = 0.5f * v[j] * (1.f + erff(v[j] * 0.70710678f));
+      for (int j = 0; j < E; ++j) v[j] = gelu_f32(v[j]);
       break;
     default:
       break;
