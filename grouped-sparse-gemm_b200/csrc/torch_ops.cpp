@@ -53,7 +53,8 @@ DeviceInfo device_info(int dev) {
   return info[dev];
 }
 
-int sm_count(const Tensor& t) { return std::max(1, device_info(t.get_device()).sm_count - g_sm_margin.load(std::memory_order_relaxed)); }
+int sm_count(int dev) { return std::max(1, device_info(dev).sm_count - g_sm_margin.load(std::memory_order_relaxed)); }
+int sm_count(const Tensor& t) { return sm_count((int)t.get_device()); }
 
 void check_arch(const Tensor& t) {
   const int v = device_info(t.get_device()).sm_version;
@@ -814,6 +815,15 @@ std::vector<std::string> group_mm_swiglu_configs() {      // csrc/ops.cu:585-589
 
 // Leave `n` SMs out of every persistent launch (see paired_nvfp4_kernels.ops.set_sm_margin).
 extern "C" __attribute__((visibility("default"))) void pnv_torch_set_sm_margin(int n) { g_sm_margin.store(std::max(0, n)); }
+
+// The SM count that the operators size their launches on device `dev` for: its SMs less the margin.
+extern "C" __attribute__((visibility("default"))) int pnv_torch_sm_count(int dev) {
+  try {
+    return sm_count(dev);
+  } catch (...) {                        // (a device that is none)
+    return 0;
+  }
+}
 
 // The torch this library was built for, looked up in the file by build.py.
 extern "C" __attribute__((visibility("default"))) const char* pnv_torch_build_id() { return PNV_TORCH_BUILD_ID; }

@@ -25,6 +25,8 @@ def _load():
                           "torch run `python grouped-sparse-gemm_b200/build.py`)") from exc
     lib.pnv_torch_set_sm_margin.argtypes = [ctypes.c_int]
     lib.pnv_torch_set_sm_margin.restype = None
+    lib.pnv_torch_sm_count.argtypes = [ctypes.c_int]
+    lib.pnv_torch_sm_count.restype = ctypes.c_int
     return lib
 
 
@@ -68,10 +70,11 @@ def group_mm_device_status():
 
 
 def linear_plan(rows, features, k, mx8=False, float_out=False, gated=False):
-    """Which kernel linear or linear_mx8 runs for these sizes on the current device: ("split", tokens of a tile, CTAs that share
-    its K) or ("pair", features of a tile)."""
+    """Which kernel linear or linear_mx8 runs for these sizes on the current device, under the SM margin that is set: ("split",
+    tokens of a tile, CTAs that share its K) or ("pair", features of a tile)."""
     v = [ctypes.c_int() for _ in range(3)]
-    _cabi.check(_lib.pnv_linear_plan(int(mx8), rows, features, k, int(float_out), int(gated), 0, *[ctypes.byref(x) for x in v]))
+    sms = _torch_lib.pnv_torch_sm_count(torch.cuda.current_device())
+    _cabi.check(_lib.pnv_linear_plan(int(mx8), rows, features, k, int(float_out), int(gated), sms, *[ctypes.byref(x) for x in v]))
     tokens, split, width = (x.value for x in v)
     return ("split", tokens, split) if tokens else ("pair", width)
 
