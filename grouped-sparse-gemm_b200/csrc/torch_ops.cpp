@@ -694,6 +694,7 @@ std::tuple<Tensor, Tensor> quant_mx8(const Tensor& x) {
   check_rows(x, "x must be bf16 [T, K] with contiguous rows");
   const int64_t T = x.size(0), K = x.size(1);
   TORCH_CHECK(K >= 1 && K % kSfBlock == 0, "K must be a multiple of ", kSfBlock, ", got ", K);
+  TORCH_CHECK(T < (1LL << 31) && K < (1LL << 31), "quant_mx8: T and K must be below 2^31, got [", T, ", ", K, "]");
   Tensor q = empty_on(x, {T, K}, at::kFloat8_e4m3fn);
   Tensor q_sf = empty_on(x, {pnv_sf_numel((int)T, (int)K, 1)}, at::kFloat8_e8m0fnu);
   const c10::cuda::CUDAGuard guard(x.device());
