@@ -38,6 +38,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "device_once.cuh"
 #include "ptx.cuh"
 #include "tensor_map.cuh"
 
@@ -729,19 +730,18 @@ int make_map_out(CUtensorMap* map, const void* base, uint64_t features, uint64_t
 // Per kernel instantiation and device, once: opt in to the large dynamic shared-memory carve-out and
 // (CTA pairs) allow the cluster launch and ask how many pairs the device runs at the same time.
 struct KernelSetup {
-  std::once_flag once[64];
-  cudaError_t err[64] = {};
-  int max_pairs[64] = {};
+  DeviceOnce once;
+  int max_pairs[kMaxDevices] = {};
 };
 
 template <class Kernel>
 int prepare_kernel(Kernel kernel, KernelSetup& ks, int threads, size_t smem, bool pair, int* max_pairs) {
   int dev = 0;
   PNV_CUDA(cudaGetDevice(&dev));
-  PNV_REQUIRE(dev >= 0 && dev < 64, "unexpected CUDA device index %d", dev);
-  std::call_once(ks.once[dev], [&] {
-    ks.err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
-    if (ks.err[dev] != cudaSuccess || !pair) return;
+  PNV_REQUIRE(dev >= 0 && dev < kMaxDevices, "unexpected CUDA device index %d", dev);
+  const cudaError_t err = ks.once(dev, [&] {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+    if (e != cudaSuccess || !pair) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * 148);
     cfg.blockDim = dim3(threads);
@@ -753,12 +753,12 @@ int prepare_kernel(Kernel kernel, KernelSetup& ks, int threads, size_t smem, boo
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    int n = 0;
-    ks.err[dev] = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
-    ks.max_pairs[dev] = n;
+    return cudaOccupancyMaxActiveClusters(&ks.max_pairs[dev], kernel, &cfg);
   });
-  if (ks.err[dev] != cudaSuccess)
-    return fail(PNV_ERR_CUDA, "group_mm kernel set-up failed: %s", cudaGetErrorString(ks.err[dev]));
+  if (err != cudaSuccess) {
+    cudaGetLastError();                  // (it is reported here, and is not to be found by whoever asks next)
+    return fail(PNV_ERR_CUDA, "group_mm kernel set-up failed: %s", cudaGetErrorString(err));
+  }
   if (max_pairs) *max_pairs = ks.max_pairs[dev];
   return PNV_OK;
 }

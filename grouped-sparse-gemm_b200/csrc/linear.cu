@@ -30,9 +30,9 @@
 #include <cuda.h>
 
 #include <algorithm>
-#include <mutex>
 
 #include "common.cuh"
+#include "device_once.cuh"
 #include "ptx.cuh"
 #include "tensor_map.cuh"
 
@@ -907,33 +907,38 @@ int rows_map(CUtensorMap* map, const void* base, uint64_t width, uint64_t rows, 
 
 constexpr int kMaxSplitLog = 3;          // clusters of 1, 2, 4 or 8 CTAs
 
-// Per kernel and device, once: the shared-memory carve-out.
-struct Setup {
-  std::once_flag once[64];
-  cudaError_t err[64] = {};
-};
-template <class Kernel>
-int prepare(Kernel kernel, Setup& s, size_t smem) {
-  int dev = 0;
+int current_device(int& dev) {
   PNV_CUDA(cudaGetDevice(&dev));
-  PNV_REQUIRE(dev >= 0 && dev < 64, "unexpected CUDA device index %d", dev);
-  std::call_once(s.once[dev], [&] { s.err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
-  if (s.err[dev] != cudaSuccess) return fail(PNV_ERR_CUDA, "linear kernel set-up failed: %s", cudaGetErrorString(s.err[dev]));
+  PNV_REQUIRE(dev >= 0 && dev < kMaxDevices, "unexpected CUDA device index %d", dev);
   return PNV_OK;
+}
+int set_up_failed(cudaError_t err) {
+  cudaGetLastError();                    // (it is reported here, and is not to be found by whoever asks next)
+  return fail(PNV_ERR_CUDA, "linear kernel set-up failed: %s", cudaGetErrorString(err));
+}
+
+// Per kernel and device, once: the shared-memory carve-out.
+template <class Kernel>
+int prepare(Kernel kernel, DeviceOnce& once, size_t smem) {
+  int dev = 0;
+  if (int rc = current_device(dev)) return rc;
+  const cudaError_t err = once(dev, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
+  return err == cudaSuccess ? PNV_OK : set_up_failed(err);
 }
 
 // Per device, once: how many clusters of 2^i CTAs run at one time.  Every kernel here fills an SM's shared memory with one CTA,
 // so one of them answers for all.
 int cluster_capacity(const int** out) {
   using C = SplitCfg<16, false>;
-  static Setup setup, asked;
-  static int clusters[64][kMaxSplitLog + 1] = {};
+  static DeviceOnce setup, asked;
+  static int clusters[kMaxDevices][kMaxSplitLog + 1] = {};
   const auto kernel = linear_split_kernel<16, false, kNothing>;
   if (int rc = prepare(kernel, setup, C::kSmem)) return rc;
   int dev = 0;
-  PNV_CUDA(cudaGetDevice(&dev));
-  std::call_once(asked.once[dev], [&] {
-    for (int i = 0; i <= kMaxSplitLog && asked.err[dev] == cudaSuccess; ++i) {
+  if (int rc = current_device(dev)) return rc;
+  const cudaError_t err = asked(dev, [&] {
+    cudaError_t e = cudaSuccess;
+    for (int i = 0; i <= kMaxSplitLog && e == cudaSuccess; ++i) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(8 << 7);
       cfg.blockDim = dim3(C::kThreads);
@@ -944,10 +949,11 @@ int cluster_capacity(const int** out) {
       attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
-      asked.err[dev] = cudaOccupancyMaxActiveClusters(&clusters[dev][i], kernel, &cfg);
+      e = cudaOccupancyMaxActiveClusters(&clusters[dev][i], kernel, &cfg);
     }
+    return e;
   });
-  if (asked.err[dev] != cudaSuccess) return fail(PNV_ERR_CUDA, "linear kernel set-up failed: %s", cudaGetErrorString(asked.err[dev]));
+  if (err != cudaSuccess) return set_up_failed(err);
   *out = clusters[dev];
   return PNV_OK;
 }
@@ -1038,7 +1044,7 @@ struct Operands {
 template <int BN, bool kMx8, int kMode>
 int launch_split(const Operands& o, const LinearArgs& a, int split, cudaStream_t stream) {
   using C = SplitCfg<BN, kMx8>;
-  static Setup setup;
+  static DeviceOnce setup;
   if (int rc = prepare(linear_split_kernel<BN, kMx8, kMode>, setup, C::kSmem)) return rc;
   CUtensorMap map_w, map_x;
   if (int rc = operand_map(&map_w, o.w, a.k_bytes, a.features, a.k_bytes, kTileRows)) return rc;
@@ -1051,7 +1057,7 @@ int launch_split(const Operands& o, const LinearArgs& a, int split, cudaStream_t
 template <bool kMx8, int kMode>
 int launch_pair(const Operands& o, LinearArgs a, int width, int sm_count, cudaStream_t stream) {
   using C = PairCfg<kMx8>;
-  static Setup setup;
+  static DeviceOnce setup;
   if (int rc = prepare(linear_pair_kernel<kMx8, kMode>, setup, C::kSmem)) return rc;
   a.tile_n = width;
   a.m_tiles = ceil_div_i(a.rows, 256);
