@@ -11,19 +11,22 @@
 //   pair     persistent; a CTA pair multiplies 256 tokens x 128 to 256 weight rows with one instruction, tokens along M, so that
 //            a thread of the epilogue holds neighbouring features of one token.  Large products.
 //
-// What bounds them, and measured times (an idle part's clock; a library product of the same operands, without bias, activation
-// and residual, in parentheses):
-//   pair     the tensor pipe, and above a few hundred microseconds the power limit: 8192 x 28672 x 4096 gated 1150 us, 1.67
-//            PFLOP/s, tensor pipe 89 % busy (1190); the same in a loop of seconds 1350 us (1390).  8-bit operands: 8192 x 7168 x
-//            2048 88 us (84), with a residual 100; in a loop 107 and 120 (103).
+// What bounds them, and measured times (a library product of the same operands, without bias, activation and residual, in
+// parentheses).  Products in a row take the SM clock from 1.9 GHz to what power allows, at once:
+//   pair     the tensor pipe at that clock: 8192 x 28672 x 4096 gated 1150 us, 1.67 PFLOP/s, 1.61 million cycles at 1.43 GHz, tensor
+//            pipe 89 % busy (1190); in a loop of seconds 1340 us, as many cycles at 1.21 GHz (1390).  8-bit operands: 8192 x 7168 x
+//            2048 88 us, 130000 cycles at 1.54 GHz (84), with a residual 100, 143000 to 146000 cycles at 1.52 GHz; in a loop 107
+//            us, 130000 cycles at 1.31 GHz (103), with a residual 120 to 123, 136000 at 1.22 GHz.
 //   split    latency where little is read: 16 x 256 x 7168 to float32 4.7 us (10.7); what a CTA takes in, 85 bytes a cycle, and
 //            the way of the partial sums, 16 bytes a cycle, otherwise: 64 x 4096 x 7168 gated on 8-bit operands 8.4 us, 30 MB
 //            (12.9).
 //
 // Accumulation.  The tensor core adds to its fp32 accumulators with truncation: over K = 7168 the sums of random products
 // come out 7e-6 too small in magnitude (relative 8e-6, against 3e-7 of fp32 arithmetic).  That is nothing beside a rounding
-// to bf16, but not for float32 results (router logits), so the split kernel lets an accumulator grow over 512 K only and
-// adds those pieces in registers: 5e-7.
+// to bf16: 8192 x 28672 x 4096, gated, is off from 64 bits by 1.658332e-3, sums in fp32 arithmetic by 1.658307e-3, and a library
+// product of these operands, activated in 64 bits, by as much as here; the other rounding is taken by 4 outputs in a thousand, where
+// fp32 arithmetic takes it by 0.7.  It would show in float32 results (router logits), so the split kernel lets an accumulator grow
+// over 512 K only there and adds those pieces in registers: 5e-7, sums of one sign 9e-7 too small (1.3e-6 at most).
 //
 // Every mbarrier wait is bounded; one that gives up records a code in g_linear_status and the roles fall through to the end,
 // where tensor memory is freed.
@@ -70,6 +73,8 @@ enum Mode : int { kNothing = 0, kActivate = 1, kGate = 2 };
 
 // ---- epilogue arithmetic -------------------------------------------------------------------------
 
+// The exponential and the reciprocal are good to 1e-7, the exponent's product is rounded first: off by 1.5e-7 for gates of unit size,
+// 9e-7 at -20, 1.7e-6 at -40 (of 1.7e-16), less than a thousandth of a bf16 unit.
 __device__ __forceinline__ float silu_f32(float g) { return g * rcp_approx(1.f + ex2_approx(g * -kLog2e)); }
 
 // v / 2 erfc(-v / sqrt(2)).  In 1 + erf a negative v cancels (6 % off at -5, nothing left from -6).  With a = |v|, t = 1 / (1 + 0.35 a):
@@ -962,7 +967,10 @@ int cluster_capacity(const int** out) {
 //
 // The constants are a fit, in units of 1/1.9 ns, to measured times of all the candidates for eight weights from 256 x 7168 to
 // 28672 x 4096 and 1 to 4096 tokens, both operand types (two thousand calls): off by a tenth on average; the candidate that it
-// picks is 1.3 % slower than the best one on average and 19 % at worst.
+// picks is 1.2 % slower than the best one on average and 18 % at worst.  Two changes came after the fit and are not in it: the split
+// kernel's bias is read ahead (a few tenths of a microsecond, for all its candidates), and pair tiles of 192 features have two
+// accumulators on 8-bit operands too (up to 5 % in several waves; an entry of their own that made them cheaper took them where
+// others are faster: K = 1024 with a residual lost 10 %).
 
 struct Plan {
   int tokens;                            // split kernel: tokens of a tile; 0: pair kernel

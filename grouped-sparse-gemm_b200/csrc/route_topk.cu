@@ -7,10 +7,13 @@
 // A warp takes a token: its keys lie in registers as unsigned numbers that order like them, every round of the selection is
 // two warp-wide integer reductions (largest key, lowest expert that has it).  Keys with a bias are sums of 32-bit roundings,
 // so two that lie closer together than those can be off might come out in the wrong order: where a selected key is that
-// close to the next one, the row is done again in 64 bits (a row in a thousand at 256 experts).
-// Bound: issue slots for many rows (16384 x 128, top-8 of softmax: 10.7 us, 554 instructions a row, 77 % of the slots), latency of
-// the reductions for few (64 x 256, top-8 of sigmoid with bias, 4 of 8 groups: 7.2 us).  One kernel for all options, keys found
-// anew every round, took 15.6 us for the former.
+// close to the next one, the row is done again in 64 bits.  That is rare where keys differ (3 rows in 10000 of 256 experts, random
+// float32 or bf16 logits and a random bias), but equal keys are as close as keys can be: bf16 logits with one bias for all make a third of
+// the rows doubtful, saturated sigmoids all of them.
+// Bound: issue slots for many rows (16384 x 128, top-8 of softmax: 10.7 us, 554 instructions a row, 77 % of the slots; 16384 x 256, top-8
+// of sigmoid with bias, 29 us, from 4 of 8 groups 52, bf16 logits 59; those with a bias of zeros 111, all rows doubtful 120), latency of
+// the reductions for few (64 x 256, the same with groups: 7.2 to 7.8 us, with a doubtful row among them 9.7, a third of them 16).  One
+// kernel for all options, keys found anew every round, took 15.6 us for the first.
 #include <algorithm>
 #include <climits>
 

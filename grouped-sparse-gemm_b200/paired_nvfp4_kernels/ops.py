@@ -40,7 +40,9 @@ def _check(cond, msg):
 
 def set_sm_margin(n):
     """Leave `n` SMs out of every persistent launch (the kernels size their grids from the SM count passed
-    in), so that a collective running on another stream finds SMs to run on.  0 restores full-width launches."""
+    in), so that a collective running on another stream finds SMs to run on.  0 restores full-width launches.  Kernels that are
+    not persistent (row kernels; linear and linear_mx8 where linear_plan says "split") still launch all their blocks and take
+    whatever SMs are free until those end."""
     _torch_lib.pnv_torch_set_sm_margin(max(0, int(n)))
 
 

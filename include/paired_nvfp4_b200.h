@@ -323,7 +323,7 @@ int pnv_group_mm_swiglu_quant(uint8_t* b_out, uint8_t* sfb_out, const uint8_t* a
  * these to the serving framework that calls it) --------------------------------------------------------------------- */
 
 /* Rows of `width` elements, x_stride apart: v = x + residual (residual and residual_out both or neither NULL),
- * n = v / sqrt(mean(v^2) + eps) * weight, in 32 bits.  Outputs, contiguous, each rounded once: residual_out bf16 = v;
+ * n = v / sqrt(mean(v^2) + eps) * weight, in 32 bits (a row whose squares add up to more than 3.4e38 comes out as zeros).  Outputs, contiguous, each rounded once: residual_out bf16 = v;
  * y bf16 = n (or NULL); q, q_sf (both or neither NULL; width a multiple of 32) = n in the 8-bit block format:
  *   q u8[rows, width] e4m3 codes; q_sf u8[pnv_sf_numel(rows, width, 1)] e8m0 scale bytes, one per 32 elements, in the scale
  *   layout of the grouped GEMM's operands (slop: 1.0).  A block's scale is the smallest power of two that brings its largest
@@ -344,8 +344,10 @@ int pnv_quant_mx8(const void* x, int64_t x_stride, int64_t rows, int k, uint8_t*
  * NULL; residual bf16, rows residual_stride apart, or NULL; out bf16 or float32, contiguous.  act_kind: PNV_ACT_NONE, _RELU,
  * _SILU, _GELU (with erf).  gated: act_kind PNV_ACT_SILU or _SITU, the rows of w (and bias) are gates and ups in 64-row blocks
  * (32 gates, their 32 ups; features a multiple of 64), out[rows, features / 2] = act(gate) * up + residual.
- * float32 outputs are good to 1e-6 of the sum's scale (partial sums are carried out of the tensor core every 512 K) and take at
- * most 65535 tiles of 128 rows. */
+ * float32 outputs are good to 1e-6 of the sum's scale, 2e-6 where all products have one sign (partial sums are carried out of the
+ * tensor core every 512 K), and take at most 65535 tiles of 128 rows.
+ * sm_count chooses the variant; the pair variant (pnv_linear_plan) launches that many CTAs, the other one as many as it has tiles,
+ * each of which fills an SM until it ends. */
 int pnv_linear(void* out, int out_is_f32, const void* x, int64_t x_stride, const void* w, const void* bias, int bias_is_f32,
                const void* residual, int64_t residual_stride, int64_t rows, int features, int k, int act_kind, int gated,
                float beta, float linear_beta, int sm_count, pnv_stream_t stream);
