@@ -75,16 +75,21 @@ __device__ __forceinline__ double exp_of(double v) { return exp(v); }
 template <class F>
 __device__ __forceinline__ F softmax_part(F l, F mx) { return mx == (F)-INFINITY ? (F)0 : l == mx ? (F)1 : exp_of(l - mx); }
 
-// The largest logit.  A NaN does not count beside a number, but where nothing is above -infinity it is the answer, so that all
-// scores of the row are NaN: as -infinity it would give the row the zeros of one that was masked.
+// The largest logit; a NaN where all scores of the row are to be NaN.  With a bias any NaN makes every key one, so that the choice
+// is none.  Without one a NaN ranks last and does not count beside a number, but where nothing is above -infinity the row must not
+// get the zeros of one that was masked.
+template <bool kBias>
 __device__ __forceinline__ float row_max(const RouteArgs& a, const void* row, int lane) {
   uint32_t m = 0;
-  for (int e = lane; e < a.experts; e += 32) m = max(m, order_of(logit_at(a, row, e)));
-  m = warp_max(m);
-  if (m > order_of(-INFINITY)) return key_of(m);
   bool nan = false;
-  for (int e = lane; e < a.experts; e += 32) nan |= isnan(logit_at(a, row, e));
-  return __any_sync(kAll, nan) ? __uint_as_float(0x7FFFFFFFu) : -INFINITY;
+  for (int e = lane; e < a.experts; e += 32) {
+    const float l = logit_at(a, row, e);
+    nan |= isnan(l);
+    m = max(m, order_of(l));
+  }
+  m = warp_max(m);
+  if ((kBias || m <= order_of(-INFINITY)) && __any_sync(kAll, nan)) return __uint_as_float(0x7FFFFFFFu);
+  return key_of(m);
 }
 template <class F>
 __device__ __forceinline__ F softmax_sum(const RouteArgs& a, const void* row, int lane, F mx) {
@@ -112,7 +117,7 @@ __device__ __forceinline__ int select(const RouteArgs& a, const void* row, const
   {
     F mx = 0, total = 1;
     if (kBias && !a.sigmoid) {
-      mx = (F)row_max(a, row, lane);
+      mx = (F)row_max<kBias>(a, row, lane);
       total = softmax_sum<F>(a, row, lane, mx);
     }
 #pragma unroll
@@ -285,7 +290,7 @@ route_topk_kernel(const RouteArgs a) {
     } else {
       float mx = -INFINITY;              // without bias and groups the first choice has it, if it is a number
       if (!kBias && !kGroups) mx = __shfl_sync(kAll, mine, 0);
-      if (kBias || kGroups || !(mx > -INFINITY)) mx = row_max(a, row, lane);
+      if (kBias || kGroups || !(mx > -INFINITY)) mx = row_max<kBias>(a, row, lane);
       if (lane < a.topk) w = softmax_part(mine, mx);
       if (!a.renormalize) {
         const float total = softmax_sum<float>(a, row, lane, mx);

@@ -57,3 +57,19 @@ def test_a_number_beside_a_nan(ops):
     for bias, renormalize in ((None, False), (torch.zeros(8, device="cuda"), True), (torch.zeros(8, device="cuda"), False)):
         w, ids = ops.route_topk(row, 3, "softmax", bias, renormalize=renormalize)
         assert bool(torch.isnan(w).all()) and ids[0].tolist() == ([3, 4, 1] if bias is None else [0, 1, 2])
+
+
+@pytest.mark.parametrize("experts,groups", [(8, 1), (64, 1), (64, 8), (300, 1), (1024, 32)])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_a_nan_that_a_bias_does_not_choose(ops, experts, groups, renormalize):
+    """With a bias every key of the row is a NaN, so the ids say nothing: no weight may look like one, wherever the NaN is."""
+    g = torch.Generator().manual_seed(experts)
+    logits = torch.randn((4, experts), generator=g)
+    logits[1, experts - 1] = logits[3, 5] = NAN
+    bias = torch.randn(experts, generator=g).cuda()
+    w, ids = ops.route_topk(logits.cuda(), 3, "softmax", bias, groups, groups, renormalize)
+    assert ids[1].tolist() == ids[3].tolist() == [0, 1, 2]
+    assert bool(torch.isnan(w[1]).all()) and bool(torch.isnan(w[3]).all())
+    for i in (0, 2):
+        alone = ops.route_topk(logits[i:i + 1].cuda(), 3, "softmax", bias, groups, groups, renormalize)
+        assert torch.equal(w[i], alone[0][0]) and torch.equal(ids[i], alone[1][0]) and bool(torch.isfinite(w[i]).all())
