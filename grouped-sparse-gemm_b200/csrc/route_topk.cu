@@ -91,6 +91,9 @@ __device__ __forceinline__ float row_max(const RouteArgs& a, const void* row, in
   if ((kBias || m <= order_of(-INFINITY)) && __any_sync(kAll, nan)) return __uint_as_float(0x7FFFFFFFu);
   return key_of(m);
 }
+// The largest of the chosen lanes' logits (none of them a NaN).
+__device__ __forceinline__ float best_of(float logit, bool chosen) { return key_of(warp_max(chosen ? order_of(logit) : 0u)); }
+
 template <class F>
 __device__ __forceinline__ F softmax_sum(const RouteArgs& a, const void* row, int lane, F mx) {
   F sum = 0;
@@ -284,13 +287,21 @@ route_topk_kernel(const RouteArgs a) {
     }
     float mine = 0.f;                    // the logit of this lane's choice: without a bias its key says it
     if (lane < a.topk) mine = kBias ? logit_at(a, row, e) : key == 1u ? __uint_as_float(0x7FFFFFFFu) : key_of(key);
+    // Renormalized scores may be smaller than 32 bits go: the chosen are then put over the best of them.
     float w = 0.f;
     if (a.sigmoid) {
-      if (lane < a.topk) w = __fdiv_rn(1.f, 1.f + expf(-mine));
+      constexpr float kSmall = -17.f;    // 1 + exp(l) is 1 in 32 bits below
+      float over = 0.f;
+      if (a.renormalize && !__any_sync(kAll, lane < a.topk && !(mine < kSmall))) {
+        over = best_of(mine, lane < a.topk);
+        if (over == -INFINITY) over = 0.f;
+      }
+      if (lane < a.topk) w = mine < kSmall ? expf(mine - over) : __fdiv_rn(1.f, 1.f + expf(-mine));
     } else {
       float mx = -INFINITY;              // without bias and groups the first choice has it, if it is a number
       if (!kBias && !kGroups) mx = __shfl_sync(kAll, mine, 0);
       if (kBias || kGroups || !(mx > -INFINITY)) mx = row_max<kBias>(a, row, lane);
+      if (kBias && a.renormalize && mx < INFINITY) mx = best_of(mine, lane < a.topk);      // (a row's infinity leaves the others 0)
       if (lane < a.topk) w = softmax_part(mine, mx);
       if (!a.renormalize) {
         const float total = softmax_sum<float>(a, row, lane, mx);

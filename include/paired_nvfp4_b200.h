@@ -371,8 +371,9 @@ int pnv_linear_device_status(int* status_out);
  * by the logit where bias is NULL; of several groups of neighbouring experts only the topk_groups best take part, ranked by the
  * sum of their two best keys (their best without a bias).  Ties go to the lower index, NaN ranks last.  Softmax scores are all NaN
  * in a row that has one: with a bias, not renormalized, or where no logit is above -infinity.  Keys that 32 bits cannot order are
- * compared in 64.  weights = scores of the chosen (without the bias), divided by their sum if renormalize, times scale; a row of
- * nothing but -infinity has weights 0 with softmax, one whose chosen scores add up to 0 when renormalized. */
+ * compared in 64.  weights = scores of the chosen (without the bias), divided by their sum if renormalize, times scale;
+ * renormalized they keep their ratios where the scores themselves are too small for 32 bits.  Scores that add up to 0 (chosen logits
+ * of nothing but -infinity; softmax, a row with an infinity that was not chosen) have weights 0. */
 #define PNV_ROUTE_MAX_EXPERTS 1024
 int pnv_route_topk(const void* logits, int logits_are_bf16, int64_t stride, int64_t rows, int experts, int topk, int sigmoid,
                    const float* bias, int groups, int topk_groups, int renormalize, float scale, float* weights,
