@@ -80,7 +80,7 @@ __device__ __forceinline__ float silu_f32(float g) { return g * rcp_approx(1.f +
 // v / 2 erfc(-v / sqrt(2)).  In 1 + erf a negative v cancels (6 % off at -5, nothing left from -6).  With a = |v|, t = 1 / (1 + 0.35 a):
 // erfc(a / sqrt(2)) / 2 = exp(-a^2 / 2) t Q(t), where t Q(t) is smooth; Q is its polynomial of degree 8 with the smallest
 // relative error over a < 14.5 (weighted least squares, 3.2e-8), above which the exponential is 0.  Off by 10 + v^2 units of 2^-23 at
-// most (v^2 / 2: what the exponent's rounding does).  4096 x 8192 x 4096 180 us, 1 + erff 178, erfcf 226.
+// most (v^2: what the exponent's rounding does).  4096 x 8192 x 4096 180 us, 1 + erff 178, erfcf 226.
 __device__ __forceinline__ float gelu_f32(float v) {
   const float a = fabsf(v) > 16.f ? 16.f : fabsf(v);           // (an infinity would meet a zero; a NaN stays one)
   const float t = rcp_approx(fmaf(a, 0.35f, 1.f));

@@ -323,7 +323,8 @@ int pnv_group_mm_swiglu_quant(uint8_t* b_out, uint8_t* sfb_out, const uint8_t* a
  * these to the serving framework that calls it) --------------------------------------------------------------------- */
 
 /* Rows of `width` elements, x_stride apart: v = x + residual (residual and residual_out both or neither NULL),
- * n = v / sqrt(mean(v^2) + eps) * weight, in 32 bits (a row whose squares add up to more than 3.4e38 comes out as zeros).  Outputs, contiguous, each rounded once: residual_out bf16 = v;
+ * n = v / sqrt(mean(v^2) + eps) * weight, in 32 bits (a row whose squares add up to more than 3.4e38 comes out as zeros).
+ * Outputs, contiguous, each rounded once: residual_out bf16 = v;
  * y bf16 = n (or NULL); q, q_sf (both or neither NULL; width a multiple of 32) = n in the 8-bit block format:
  *   q u8[rows, width] e4m3 codes; q_sf u8[pnv_sf_numel(rows, width, 1)] e8m0 scale bytes, one per 32 elements, in the scale
  *   layout of the grouped GEMM's operands (slop: 1.0).  A block's scale is the smallest power of two that brings its largest
